@@ -82,7 +82,29 @@ SIGNATURES = {
     "ct_engine_step_times": (_int, [_vp, _vp, _int]),
     "ct_engine_set_prompt": (_int, [_vp, _vp, _int]),
     "ct_engine_last_logits": (_int, [_vp, _vp, _vp, _vp, _int]),
+    # 8-bit paged cache (include/ct_kv8.h)
+    "ct_kv8_append": (_int, [_vp, _int, _vp, _vp, _int, _vp, _int, _int, _vp, _int, _vp]),
+    "ct_kv8_attn": (_int, [_vp, _int, _vp, _vp, _int, _vp, _int, _int, _int, _vp, _int, _int, _int, _flt, _int, _int,
+                           _int, _vp, _sz, _vp]),
+    "ct_kv8_attn_ws_bytes": (_sz, [_vp, _vp, _int, _int, _int, _int, _int, _int, _int, _int]),
+    "ct_kv8_reserve": (_int, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    "ct_kv8_fork": (_int, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ct_kv8_free": (_int, [_vp, _vp, _vp, _int, _vp]),
+    "ct_kv8_trim": (_int, [_vp, _vp, _int, _int, _vp]),
+    "ct_kv8_compact": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ct_kv8_copy_pages": (_int, [_vp, _vp, _vp, _int, _vp]),
+    "ct_kv8_pages_ws_bytes": (_sz, [_vp, _int]),
+    "ct_kv8_status": (_int, []),
 }
+
+
+class KV8Cache(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("refs", _vp), ("n_pages", _int), ("n_layers", _int),
+                ("kv_heads", _int), ("head_dim", _int), ("format", _int)]
+
+
+class KV8Seqs(ctypes.Structure):
+    _fields_ = [("table", _vp), ("len", _vp), ("n_seqs", _int), ("table_stride", _int)]
 
 
 class EngineConfig(ctypes.Structure):

@@ -5,3 +5,4 @@
 #include "backend_abi.cu"
 #include "engine.cu"
 #include "noalloc.cu"
+#include "kv8.cu"

@@ -42,6 +42,7 @@ enum {
     CT_STATUS_TIMEOUT_FREE = 3,  // a stage was never released
     CT_STATUS_BAD_ARG = 4,       // a kernel saw an out-of-range index and skipped it
     CT_STATUS_TIMEOUT_GRID = 5,  // a grid barrier or a split-K tile counter of the persistent step never filled
+    CT_STATUS_NO_PAGE = 6,       // no free page was left in an 8-bit cache's pool
 };
 // Defined here: the library is built as one translation unit (ct_b200.cu).
 __device__ int g_ct_status = 0;

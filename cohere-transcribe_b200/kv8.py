@@ -1,0 +1,237 @@
+"""The 8-bit paged K/V cache of include/ct_kv8.h on torch tensors.
+
+`Cache` and `Seqs` hold the tensors a caller owns; the methods check their
+arguments and call the C entry points on the current torch stream of the
+cache's device.  They never synchronise (`status` does).
+
+    cache = Cache.empty(n_pages, n_layers, kv_heads, head_dim, "e4m3")
+    seqs = Seqs.empty(n_seqs, max_pages)
+    cache.reserve(seqs, add)                            # room for this step's rows
+    for layer in range(n_layers):
+        cache.append(layer, seqs, k, v)                 # [n_seqs, kv_heads, head_dim], one row each
+        out = cache.attend(layer, seqs, q)              # [n_seqs, heads, head_dim]
+    cache.free(seqs)
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import abi
+
+ROWS = 16                                # token rows of a page (CT_KV8_ROWS)
+FORMATS = {"e4m3": 0, "int8": 1}
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+class KV8Error(RuntimeError):
+    """A ct_kv8_* call returned an error code (`code`)."""
+
+    def __init__(self, name, code):
+        super().__init__(f"{name} failed: {code}")
+        self.code = code
+
+
+def _check(rc, name):
+    if rc != 0:
+        raise KV8Error(name, rc)
+
+
+def _need(cond, what):
+    if not cond:
+        raise ValueError(what)
+
+
+def _ints(t, shape, device, what):
+    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_contiguous() and t.device == device
+          and (shape is None or tuple(t.shape) == shape), f"{what}: a contiguous int32 tensor"
+          + (f" {list(shape)}" if shape is not None else "") + f" on {device}")
+    return t.data_ptr()
+
+
+class Seqs:
+    """Sequences: page table [n_seqs, max_pages] and lengths [n_seqs], int32."""
+
+    def __init__(self, table, lens):
+        _need(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, "table: [n_seqs, max_pages]")
+        p = _ints(table, None, table.device, "table")
+        q = _ints(lens, (table.shape[0],), table.device, "lens")
+        self.table, self.lens = table, lens
+        self.n, self.max_pages = table.shape
+        self.c = abi.KV8Seqs(p, q, self.n, self.max_pages)
+        self.ref = ctypes.addressof(self.c)
+
+    @classmethod
+    def empty(cls, n_seqs, max_pages, device="cuda"):
+        return cls(torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(n_seqs, dtype=torch.int32, device=device))
+
+
+class Cache:
+    """A pool of pages: codes uint8 [pages, layers, 2, kv_heads, 16, head_dim], scales float32
+    [pages, layers, 2, kv_heads], refs int32 [pages] (None: the caller assigns pages itself)."""
+
+    def __init__(self, codes, scales, refs=None, fmt="e4m3"):
+        _need(codes.dtype == torch.uint8 and codes.dim() == 6 and codes.is_contiguous() and codes.is_cuda
+              and codes.shape[2] == 2 and codes.shape[4] == ROWS and codes.shape[5] in (64, 128),
+              "codes: a contiguous uint8 tensor [pages, layers, 2, kv_heads, 16, 64 or 128] on a GPU")
+        _need(scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == codes.shape[:4]
+              and scales.device == codes.device, "scales: a contiguous float32 tensor [pages, layers, 2, kv_heads]")
+        _need(fmt in FORMATS, "fmt: 'e4m3' or 'int8'")
+        self.codes, self.scales, self.refs, self.fmt = codes, scales, refs, fmt
+        self.n_pages, self.n_layers, _, self.kv_heads, _, self.head_dim = codes.shape
+        self.device = codes.device
+        r = _ints(refs, (self.n_pages,), self.device, "refs") if refs is not None else None
+        self.lib = abi.load()
+        self.c = abi.KV8Cache(codes.data_ptr(), scales.data_ptr(), r, self.n_pages, self.n_layers, self.kv_heads,
+                              self.head_dim, FORMATS[fmt])
+        self.ref = ctypes.addressof(self.c)
+
+    @classmethod
+    def empty(cls, n_pages, n_layers, kv_heads, head_dim, fmt="e4m3", device="cuda"):
+        shape = (n_pages, n_layers, 2, kv_heads)
+        return cls(torch.zeros(*shape, ROWS, head_dim, dtype=torch.uint8, device=device),
+                   torch.zeros(*shape, device=device), torch.zeros(n_pages, dtype=torch.int32, device=device), fmt)
+
+    # ---- helpers
+    def _call(self, name, *args):
+        """The C call with this device current, on its current torch stream."""
+        if torch.cuda.current_device() == self.device.index:
+            rc = getattr(self.lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                rc = getattr(self.lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+        _check(rc, name)
+
+    def _seqs(self, s):
+        _need(s.table.device == self.device, f"the sequences are not on {self.device}")
+        return s.ref
+
+    def _layer(self, layer):
+        _need(0 <= layer < self.n_layers, f"layer: 0 .. {self.n_layers - 1}")
+        return layer
+
+    def _rows(self, x, heads, what):
+        """Row stride of [rows, heads, head_dim] with each row contiguous."""
+        _need(x.dim() == 3 and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads)
+              and x.shape[0] > 0 and x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == self.head_dim)
+              and x.dtype in _TYPES and x.device == self.device,
+              f"{what}: float32 or bfloat16 [rows, {heads or 'heads'}, {self.head_dim}] on {self.device}, rows contiguous")
+        ld = x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+        _need(ld >= x.shape[1] * x.shape[2] and ld * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0,
+              f"{what}: rows of 16-byte alignment that do not overlap")
+        return ld
+
+    def _ws(self, ws, need):
+        if need == 0:
+            return None, None, 0
+        if ws is None:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        _need(ws.dtype == torch.uint8 and ws.is_contiguous() and ws.device == self.device and ws.numel() >= need,
+              f"ws: a contiguous uint8 tensor of at least {need} bytes on {self.device}")
+        return ws, ws.data_ptr(), ws.numel()
+
+    def _starts(self, seqs, rows, row_start, max_rows):
+        if row_start is None:
+            _need(max_rows == 1 and rows >= seqs.n, "without row_start: max_rows 1 and a row for each sequence")
+            return None
+        return _ints(row_start, (seqs.n + 1,), self.device, "row_start")
+
+    # ---- operators
+    def append(self, layer, seqs, k, v, row_start=None, max_rows=1):
+        """Write the rows k, v [rows, kv_heads, head_dim] (ct_kv8_append)."""
+        ldk, ldv = self._rows(k, self.kv_heads, "k"), self._rows(v, self.kv_heads, "v")
+        _need(k.dtype == v.dtype and k.shape == v.shape, "k and v: the same shape and type")
+        rs = self._starts(seqs, k.shape[0], row_start, max_rows)
+        self._call("ct_kv8_append", self.ref, self._layer(layer), self._seqs(seqs), k.data_ptr(), ldk, v.data_ptr(),
+                   ldv, _TYPES[k.dtype], rs, max_rows)
+
+    def _attend_ws_bytes(self, seqs, q, max_rows, max_len, causal, window, sinks):
+        return self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, _TYPES[q.dtype], q.shape[0], max_rows, max_len,
+                                             q.shape[1], int(causal), window, sinks)
+
+    def attend_workspace(self, seqs, q, max_rows=1, max_len=None, causal=True, window=0, sinks=0):
+        """A workspace for `attend` calls of these sizes (one per stream that may run them at the same time)."""
+        self._rows(q, None, "q")
+        n = self._attend_ws_bytes(seqs, q, max_rows, seqs.max_pages * ROWS if max_len is None else max_len, causal,
+                                  window, sinks)
+        return torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
+
+    def attend(self, layer, seqs, q, out=None, row_start=None, max_rows=1, max_len=None, causal=True, window=0,
+               sinks=0, scale=None, ws=None):
+        """Attention of q [rows, heads, head_dim] over the sequences' pages (ct_kv8_attn); max_len bounds their
+        lengths (default: the table's width)."""
+        ldq = self._rows(q, None, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        ldo = self._rows(out, q.shape[1], "out")
+        _need(out.dtype == q.dtype and out.shape == q.shape, "out: q's shape and type")
+        _need(q.shape[1] % self.kv_heads == 0, "heads: a multiple of kv_heads")
+        rs = self._starts(seqs, q.shape[0], row_start, max_rows)
+        max_len = seqs.max_pages * ROWS if max_len is None else max_len
+        need = self._attend_ws_bytes(seqs, q, max_rows, max_len, causal, window, sinks)
+        ws, p, n = self._ws(ws, need)
+        self._call("ct_kv8_attn", self.ref, self._layer(layer), self._seqs(seqs), q.data_ptr(), ldq, out.data_ptr(),
+                   ldo, _TYPES[q.dtype], q.shape[0], rs, max_rows, max_len, q.shape[1],
+                   self.head_dim ** -0.5 if scale is None else scale, int(causal), window, sinks, p, n)
+        return out
+
+    def pages_workspace(self, seqs):
+        """A workspace for `reserve` and `compact` of seqs, and for `fork` into them."""
+        n = self.lib.ct_kv8_pages_ws_bytes(self.ref, seqs.n)
+        return torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
+
+    def _pages_ws(self, seqs, ws):
+        return self._ws(ws, self.lib.ct_kv8_pages_ws_bytes(self.ref, seqs.n))
+
+    def reserve(self, seqs, add, ws=None):
+        """lens += add, with pages for the new rows (ct_kv8_reserve)."""
+        a = _ints(add, (seqs.n,), self.device, "add")
+        ws, p, n = self._pages_ws(seqs, ws)
+        self._call("ct_kv8_reserve", self.ref, self._seqs(seqs), a, p, n)
+
+    def fork(self, src, parents, dst, ws=None):
+        """Sequence i of dst continues src[parents[i]] (ct_kv8_fork)."""
+        a = _ints(parents, (dst.n,), self.device, "parents")
+        ws, p, n = self._pages_ws(dst, ws)
+        self._call("ct_kv8_fork", self.ref, self._seqs(src), a, self._seqs(dst), p, n)
+
+    def free(self, seqs, which=None):
+        """Release all sequences, or those listed in which (ct_kv8_free)."""
+        w = None if which is None else _ints(which, None, self.device, "which")
+        self._call("ct_kv8_free", self.ref, self._seqs(seqs), w, 0 if which is None else which.numel())
+
+    def trim(self, seqs, window, sinks=0):
+        """Release the pages that a window has passed (ct_kv8_trim)."""
+        self._call("ct_kv8_trim", self.ref, self._seqs(seqs), window, sinks)
+
+    def compact(self, seqs, refs_out=None, table_out=None, n_live=None, ws=None):
+        """Move the live pages to the pool's start (ct_kv8_compact); in place unless outputs are given."""
+        _need(self.refs is not None, "the cache has no refs")
+        refs_out = self.refs if refs_out is None else refs_out
+        table_out = seqs.table if table_out is None else table_out
+        r = _ints(refs_out, (self.n_pages,), self.device, "refs_out")
+        t = _ints(table_out, tuple(seqs.table.shape), self.device, "table_out")
+        k = None if n_live is None else _ints(n_live, (1,), self.device, "n_live")
+        ws, p, n = self._pages_ws(seqs, ws)
+        self._call("ct_kv8_compact", self.ref, self._seqs(seqs), r, t, k, p, n)
+
+    def copy_pages(self, src, dst):
+        """Copy pages src[i] -> dst[i] (ct_kv8_copy_pages)."""
+        a, b = _ints(src, None, self.device, "src"), _ints(dst, None, self.device, "dst")
+        _need(src.numel() == dst.numel(), "src and dst: the same number of pages")
+        self._call("ct_kv8_copy_pages", self.ref, a, b, src.numel())
+
+    def status(self):
+        """Read and clear the device status word (waits for the device)."""
+        with torch.cuda.device(self.device):
+            return self.lib.ct_kv8_status()
+
+    def values(self, layer, seqs, s, n=None):
+        """K and V of the first n (default: all) rows of sequence s as float32 [n, kv_heads, head_dim] each."""
+        n = int(seqs.lens[s]) if n is None else n
+        pages = seqs.table[s, :(n + ROWS - 1) // ROWS].long()
+        x = self.codes[pages, layer].view(torch.float8_e4m3fn if self.fmt == "e4m3" else torch.int8).float()
+        x = (x * self.scales[pages, layer][..., None, None]).permute(1, 0, 3, 2, 4).flatten(1, 2)[:, :n]
+        return x[0], x[1]
