@@ -83,7 +83,7 @@ SIGNATURES = {
     "ct_engine_set_prompt": (_int, [_vp, _vp, _int]),
     "ct_engine_last_logits": (_int, [_vp, _vp, _vp, _vp, _int]),
     # 8-bit paged cache (include/ct_kv8.h)
-    "ct_kv8_append": (_int, [_vp, _int, _vp, _vp, _int, _vp, _int, _int, _vp, _int, _vp]),
+    "ct_kv8_append": (_int, [_vp, _int, _vp, _vp, _int, _vp, _int, _int, _int, _vp, _int, _vp]),
     "ct_kv8_attn": (_int, [_vp, _int, _vp, _vp, _int, _vp, _int, _int, _int, _vp, _int, _int, _int, _flt, _int, _int,
                            _int, _vp, _sz, _vp]),
     "ct_kv8_attn_ws_bytes": (_sz, [_vp, _vp, _int, _int, _int, _int, _int, _int, _int, _int]),

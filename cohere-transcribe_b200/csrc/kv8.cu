@@ -1,7 +1,11 @@
 // kv8.cu -- the 8-bit paged K/V cache (include/ct_kv8.h): rows written into
 // pages, the pages' bookkeeping, and the C entry points.
+#include <algorithm>
+#include <atomic>
+
 #include "kv8.cuh"
 #include "kv8_attn.cuh"
+#include "kv8_many.cuh"
 
 namespace ct {
 namespace kv8 {
@@ -13,7 +17,7 @@ namespace kv8 {
 struct AppendArgs {
     Pool p;
     const int *table, *len, *row_start;
-    int stride, max_rows, n_seqs, layer;
+    int stride, n_rows, max_rows, n_seqs, layer;
     const void *src[2];
     int ld[2];
     int items;   // blocks x heads x 2 of a sequence, at most
@@ -25,7 +29,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
     const int s = blockIdx.y, lane = threadIdx.x & 31;
     const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (item >= a.items) return;
-    const RowSpan sp = row_span(a.len, a.row_start, s, INT_MAX, a.max_rows, a.stride * ROWS);
+    const RowSpan sp = row_span(a.len, a.row_start, s, a.n_rows, a.max_rows, a.stride * ROWS);
     if ((sp.n == 0 && sp.ok) || (!a.row_start && sp.len <= 0)) return;   // no row
     if (!sp.ok || sp.n > sp.len) {
         if (lane == 0) set_status(CT_STATUS_BAD_ARG);
@@ -444,7 +448,8 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const Pool p, const int
 static bool good_cache(const ct_kv8_cache *c) {
     return c && c->codes && c->scales && c->n_pages > 0 && c->n_layers > 0 && c->n_layers <= 4096 && c->kv_heads > 0 &&
            c->kv_heads <= 4096 && (c->head_dim == 64 || c->head_dim == 128) &&
-           (c->format == CT_KV8_E4M3 || c->format == CT_KV8_INT8) && (reinterpret_cast<uintptr_t>(c->codes) & 15) == 0 &&
+           (c->format == CT_KV8_E4M3 || c->format == CT_KV8_INT8) &&
+           (long long)c->n_pages * c->n_layers * c->kv_heads < (1ll << 30) &&   // blocks are numbered in 31 bits (reinterpret_cast<uintptr_t>(c->codes) & 15) == 0 &&
            (reinterpret_cast<uintptr_t>(c->scales) & 3) == 0;
 }
 static bool good_seqs(const ct_kv8_seqs *s) {
@@ -481,9 +486,39 @@ static int launch(void (*k)(P...), dim3 grid, int threads, size_t smem, cudaStre
     return CT_OK;
 }
 
+// The pool as [blocks][16 rows][dim] bytes, boxes of one block, swizzled.
+static int pool_map(CUtensorMap *map, const Pool &p) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::atomic<Encode> encode{nullptr};
+    Encode f = encode.load(std::memory_order_acquire);
+    if (!f) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess || !fn) {
+            cudaGetLastError();
+            return CT_EDEVICE;
+        }
+        f = reinterpret_cast<Encode>(fn);
+        encode.store(f, std::memory_order_release);
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t)p.dim, (cuuint64_t)ROWS, (cuuint64_t)p.n_pages * p.page_scales()};
+    const cuuint64_t strides[2] = {(cuuint64_t)p.dim, (cuuint64_t)p.dim * ROWS};
+    const cuuint32_t box[3] = {(cuuint32_t)p.dim, (cuuint32_t)ROWS, 1}, one[3] = {1, 1, 1};
+    return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, p.codes, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             p.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? CT_OK : CT_EDEVICE;
+}
+
 // ---- attention: which kernel, which tiles, which pieces
+#ifndef CT_KV8_FEW
+#define CT_KV8_FEW 64   // query rows of a sequence and kv head up to which few_kernel is taken
+#endif
 struct AttnPlan {
-    int mt;          // few_kernel: tiles of 8 query rows per CTA
+    int mt;          // few_kernel: tiles of 8 query rows per CTA; 0: many_kernel
+    int tile;        // query rows of a CTA
     int tiles;       // row tiles of a sequence and kv head, at most
     int chunk, max_chunks;
     size_t ws;
@@ -495,17 +530,26 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
     if (heads <= 0 || heads % c->kv_heads || heads / c->kv_heads > 1024) return false;
     if (window < 0 || window > (1 << 30) || sinks < 0 || sinks > (1 << 30) || (window && !causal)) return false;
     const long long rows = (long long)max_rows * (heads / c->kv_heads);   // query rows per kv head
-    pl.mt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    const int tile = 8 * pl.mt;
-    const long long tiles = (rows + tile - 1) / tile;
+    const int group = heads / c->kv_heads;
+    pl.mt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= CT_KV8_FEW ? 4 : 0;
+    pl.tile = pl.mt ? 8 * pl.mt : type == CT_KV8_F32 ? 128 : 256;
+    const long long tiles = (rows + pl.tile - 1) / pl.tile;
     long long list = pages_of(std::min<long long>(max_len, (long long)s->table_stride * ROWS));
     if (window) {
-        const long long span = (long long)window + tile / (heads / c->kv_heads) + 1;
+        const long long span = (long long)window + pl.tile / group + 1;
         list = std::min(list, pages_of(sinks) + (span + ROWS - 1) / ROWS + 1);
     }
-    int chunk = 64;
-    while (chunk > 4 && s->n_seqs * (long long)c->kv_heads * tiles * ((list + chunk - 1) / chunk) < 592) chunk /= 2;
-    pl.chunk = chunk;
+    const long long ctas = s->n_seqs * (long long)c->kv_heads * tiles;
+    long long chunk;
+    if (pl.mt) {
+        chunk = FEW_CHUNK;
+        while (chunk > 4 && ctas * ((list + chunk - 1) / chunk) < 592) chunk /= 2;
+    } else {
+        // whole key tiles; one piece once the tiles alone give every SM a CTA
+        const long long pieces = std::min(std::max(1ll, 148 / ctas), std::max(1ll, list / (4 * KB)));
+        chunk = ((list + pieces - 1) / pieces + KB - 1) / KB * KB;
+    }
+    pl.chunk = (int)chunk;
     pl.tiles = (int)tiles;
     pl.max_chunks = (int)((list + chunk - 1) / chunk);
     if (tiles * pl.max_chunks > INT_MAX) return false;
@@ -515,19 +559,35 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
 
 template <typename T, int D, int FMT, int MT>
 static int launch_few(const AttnArgs &a, const AttnPlan &pl, cudaStream_t st) {
-    constexpr size_t smem = sizeof(FewSmem<D, MT>);
+    constexpr size_t smem = sizeof(FewSmem<T, D, MT>) + 1024;
+    CUtensorMap map;
+    if (pool_map(&map, a.p) != CT_OK) return CT_EDEVICE;
     if (smem > 48 * 1024 &&
         cudaFuncSetAttribute(few_kernel<T, D, FMT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
         cudaGetLastError();
         return CT_EDEVICE;
     }
-    int rc = launch(few_kernel<T, D, FMT, MT>, dim3(pl.max_chunks * pl.tiles, a.p.heads, a.n_seqs), 128, smem, st, false, a);
+    int rc = launch(few_kernel<T, D, FMT, MT>, dim3(pl.max_chunks * pl.tiles, a.p.heads, a.n_seqs), 128, smem, st, false, map, a);
     if (rc == CT_OK && pl.max_chunks > 1)
         rc = launch(join_kernel<T, D>, dim3(pl.tiles, a.p.heads, a.n_seqs), 256, 0, st, true, a, 8 * MT);
     return rc;
 }
 template <typename T, int D, int FMT>
+static int launch_many(const AttnArgs &a, const AttnPlan &pl, cudaStream_t st) {
+    constexpr size_t smem = sizeof(ManySmem<D>) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    if (cudaFuncSetAttribute(many_kernel<T, D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+        cudaGetLastError();
+        return CT_EDEVICE;
+    }
+    int rc = launch(many_kernel<T, D, FMT>, dim3(pl.max_chunks * pl.tiles, a.p.heads, a.n_seqs), MANY_THREADS, smem, st, false, a);
+    if (rc == CT_OK && pl.max_chunks > 1)
+        rc = launch(join_kernel<T, D>, dim3(pl.tiles, a.p.heads, a.n_seqs), 256, 0, st, true, a, pl.tile);
+    return rc;
+}
+template <typename T, int D, int FMT>
 static int launch_attn(const AttnArgs &a, const AttnPlan &pl, cudaStream_t st) {
+    if (pl.mt == 0) return launch_many<T, D, FMT>(a, pl, st);
     if (pl.mt == 1) return launch_few<T, D, FMT, 1>(a, pl, st);
     if (pl.mt == 2) return launch_few<T, D, FMT, 2>(a, pl, st);
     return launch_few<T, D, FMT, 4>(a, pl, st);
@@ -568,17 +628,19 @@ static bool good_ws(const void *ws) { return ws && (reinterpret_cast<uintptr_t>(
 using namespace ct::kv8;
 
 extern "C" int ct_kv8_append(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const void *k, int ldk,
-                             const void *v, int ldv, int type, const int *row_start, int max_rows, void *stream) {
+                             const void *v, int ldv, int type, int n_rows, const int *row_start, int max_rows,
+                             void *stream) {
     if (!good_cache(c) || !good_seqs(s) || layer < 0 || layer >= c->n_layers) return CT_EINVAL;
     if (type != CT_KV8_F32 && type != CT_KV8_BF16) return CT_EINVAL;
     const long long width = (long long)c->kv_heads * c->head_dim;
     if (!good_rows(k, ldk, width, type) || !good_rows(v, ldv, width, type)) return CT_EINVAL;
-    if (max_rows <= 0 || max_rows > (1 << 20) || (!row_start && max_rows != 1)) return CT_EINVAL;
+    if (n_rows <= 0 || max_rows <= 0 || max_rows > (1 << 20)) return CT_EINVAL;
+    if (!row_start && (max_rows != 1 || n_rows < s->n_seqs)) return CT_EINVAL;
     if (cudaPeekAtLastError() != cudaSuccess) return CT_EDEVICE;
     AppendArgs a = {};
     a.p = pool_of(c);
     a.table = s->table; a.len = s->len; a.row_start = row_start;
-    a.stride = s->table_stride; a.max_rows = max_rows; a.n_seqs = s->n_seqs; a.layer = layer;
+    a.stride = s->table_stride; a.n_rows = n_rows; a.max_rows = max_rows; a.n_seqs = s->n_seqs; a.layer = layer;
     a.src[0] = k; a.src[1] = v;
     a.ld[0] = ldk; a.ld[1] = ldv;
     const long long items = ((max_rows + ROWS - 2) / ROWS + 1) * 2ll * c->kv_heads;

@@ -61,11 +61,29 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
+// Chunk (16 bytes) that TMA's swizzle moves chunk 0 of `row` to, rows of D bytes:
+// 128-byte rows take the 128-byte pattern, 64-byte rows the 64-byte one.
+template <int D>
+__device__ __forceinline__ int swz(int row) { return D == 128 ? row & 7 : (row >> 1) & 3; }
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // The power of two that brings the largest magnitude of a row into [1, 2); 1 for
 // zero and non-finite ones.
 __device__ __forceinline__ float row_pow2(float amax) {
     const int e = (int)(__float_as_uint(amax) >> 23);
-    return (e == 0 || e == 255) ? 1.0f : __uint_as_float((uint32_t)min(max(254 - e, 1), 254) << 23);
+    return (e == 0 || e == 255) ? 1.0f : __uint_as_float((uint32_t)min(max(254 - e, 1), 253) << 23);
+}
+// 1 / x of a power of two in [2^-126, 2^126], without a division.
+__device__ __forceinline__ float inv_pow2(float x) { return __uint_as_float(0x7F000000u - __float_as_uint(x)); }
+// The power of two that O is held in for block scales up to vmax.
+__device__ __forceinline__ float o_unit(float vmax) {
+    return fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7F800000u), 1.1754944e-38f), 8.5070592e37f);
 }
 
 template <typename T>
@@ -95,36 +113,60 @@ __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d)
 // One CTA per (piece of `chunk` pages, kv head and tile of 8 MT query rows,
 // sequence); the rows of a tile are (query row, head of the group) pairs, so the
 // heads that share a kv head read its codes once.  Each of the four warps takes
-// every fourth page with an online softmax of its own; the warps join through
-// shared memory at the end.
+// every fourth page, two at a time, with an online softmax of its own; the warps
+// join through shared memory at the end.
 //
-// Products on the tensor cores (m16n8k16, fp16 in, fp32 sums): codes are exact
-// in fp16, and the 16 rows of the MMA hold 8 query rows twice, as the high and
-// the low fp16 part of the (power-of-two scaled) query, so the sum of both
-// halves carries the query with 22 bits at no extra instruction.  The
-// probabilities go the same way into P.V.  Lane (g, t) = (lane / 4, lane % 4)
-// holds of each operand what one or two 16-byte loads of a key row give it: a
-// product over d does not care in which order the d come, so K fragments take
-// 4 consecutive bytes per MMA, and the columns of V fragments are the 16 (8)
-// consecutive dims that lane group g loaded.  Codes go from global memory to
-// registers to the MMA, the next page's loads in flight meanwhile.
-template <int D, int MT>
+// Products on the warp-level tensor path (m16n8k16, fp16 in, fp32 sums) with the
+// cache as the 16-row operand and the query rows as the 8 columns, so that no
+// half of the MMA is empty: S^T = K Q^T (16 keys x 8 rows) and O^T += V^T P^T
+// (16 dims x 8 rows).  Codes are exact in fp16.  fp32 queries and probabilities
+// are two fp16 each (two MMAs into the same sums), bf16 ones one (queries are
+// exact: each row is scaled by a power of two).  Lane (g, t) = (lane / 4,
+// lane % 4) gets of K and V what one or two 16-byte loads of a row hold: a
+// product over d does not care in which order the d come, so K's fragments take
+// 4 consecutive bytes per MMA, and V's 16 rows are neighbouring dims of the 16
+// (8) that lane group g loaded.  P^T comes from S^T by 8 x 8 transposes.
+//
+// The reference of a row's exponentials moves only when some score passes it by
+// 2^THR, so most pages need one vote and no shuffles; V's block scale goes into
+// the probabilities, relative to a power of two E per row that O is held in and
+// that moves the same way.  P = 2^(x - reference + OFF) vs / E <= 2^15.
+//
+// Each warp keeps FEW_STAGES pages in flight through a ring of its own, one TMA
+// copy per K and V block; TMA's swizzle spreads both access patterns over all
+// banks.
+constexpr int FEW_STAGES = 4;             // pages in flight per warp
+constexpr int FEW_CHUNK = 128;            // pages of a piece at most: a lane of each warp per page
+
+template <typename T, int D, int MT>
 struct FewSmem {
+    static constexpr int QW = sizeof(T) == 4 ? 4 : 2;
     union {
-        uint4 q[MT][D / 16][32];          // A fragments: hi, lo, hi, lo
-        float o[4][8 * MT][D];
+        uint8_t kv[4][FEW_STAGES][2][ROWS * D];   // per warp: K and V blocks as TMA wrote them
+        float o[4][8 * MT][D];                    // the warps' results, for the join
     };
+    uint32_t q[MT][D / 16][32][QW];       // B fragments: high parts, low parts
+    float qf[8 * MT];                     // per row: scale_log2 / its power of two
     float m[4][8 * MT], l[4][8 * MT];
+    uint64_t full[4][FEW_STAGES];
 };
 
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 template <typename T, int D, int FMT, int MT>
-__global__ void __launch_bounds__(128) few_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(128, MT <= 2 ? 3 : 2) few_kernel(const __grid_constant__ CUtensorMap map, const AttnArgs a) {
+    constexpr bool TWO = sizeof(T) == 4;
     constexpr int KC = D / 64;            // 16-byte loads per key row and lane
-    constexpr int KS = D / 16;            // MMA steps over the head dim
-    constexpr int NJ = D / 8;             // MMA column tiles over the head dim
+    constexpr int KS = D / 16;            // MMA steps of Q.K
+    constexpr int NJ = D / 16;            // MMA row tiles of P.V
     constexpr int VB = D / 8;             // V bytes per key and lane
-    extern __shared__ __align__(16) uint8_t few_raw[];
-    FewSmem<D, MT> &sm = *reinterpret_cast<FewSmem<D, MT> *>(few_raw);
+    constexpr float THR = 4.0f, OFF = 7.0f;
+    extern __shared__ __align__(1024) uint8_t few_raw[];
+    FewSmem<T, D, MT> &sm = *reinterpret_cast<FewSmem<T, D, MT> *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int s = blockIdx.z, hk = blockIdx.y, tile = blockIdx.x / a.max_chunks, piece = blockIdx.x % a.max_chunks;
     pdl_trigger();
@@ -142,10 +184,42 @@ __global__ void __launch_bounds__(128) few_kernel(const AttnArgs a) {
     const int pieces = max(1, (list.n + a.chunk - 1) / a.chunk);
     if (piece >= pieces) return;
 
-    // queries -> A fragments: warp w prepares row tile w (w < MT)
-    float qf[MT];                         // per row g of each tile: scale_log2 / row's power of two
-    for (int mt = 0; mt < MT; ++mt) {
-        const int m = m0 + mt * 8 + g;
+    // this warp's pages: lane i holds the i-th one's number and block scales
+    const int e0 = piece * a.chunk + warp, e1 = min(list.n, (piece + 1) * a.chunk);
+    const int mine = e1 > e0 ? (e1 - e0 + 3) / 4 : 0;
+    int page = -1;
+    if (lane < mine) page = a.table[(size_t)s * a.stride + list.at(e0 + 4 * lane)];
+    if (lane == 0) {
+        for (int i = 0; i < FEW_STAGES; ++i) mbar_init(&sm.full[warp][i], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    float ks = 0.0f, vs = 0.0f;
+    if (lane < mine) {
+        if (a.p.has(page)) {
+            const size_t b = a.p.block(page, a.layer, 0, hk);
+            ks = a.p.scales[b];
+            vs = a.p.scales[b + a.p.heads];
+        } else {
+            set_status(CT_STATUS_BAD_ARG);   // its rows count as not there
+            page = -1;
+        }
+    }
+    auto issue = [&](int i) {             // page i of this warp -> stage i % FEW_STAGES
+        const int p = __shfl_sync(0xffffffffu, page, i & 31);
+        if (i < mine && p >= 0 && lane == 0) {
+            const int st = i % FEW_STAGES, b = (int)a.p.block(p, a.layer, 0, hk);
+            mbar_expect_tx(&sm.full[warp][st], 2 * ROWS * D);
+            tma_load_3d(sm.kv[warp][st][0], &map, &sm.full[warp][st], 0, 0, b);
+            tma_load_3d(sm.kv[warp][st][1], &map, &sm.full[warp][st], 0, 0, b + a.p.heads);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < FEW_STAGES; ++i) issue(i);
+
+    // queries -> B fragments: tile mt by warp mt
+    if (warp < MT) {
+        const int mt = warp, m = m0 + mt * 8 + g;
         float amax = 0.0f;
         float v[KC][2][8];
 #pragma unroll
@@ -156,7 +230,7 @@ __global__ void __launch_bounds__(128) few_kernel(const AttnArgs a) {
                 for (int j = 0; j < 8; ++j) v[i][e][j] = 0.0f;
                 if (m < M) {
                     const T *qp = static_cast<const T *>(a.q) + (size_t)(sp.first + m / G) * a.ldq +
-                                  (size_t)(hk * G + m % G) * D + (t + 4 * i) * 16 + e * 8;
+                                  (size_t)(hk * G + m % G) * D + (KC * t + i) * 16 + e * 8;
                     load8(qp, v[i][e]);
                 }
 #pragma unroll
@@ -165,201 +239,264 @@ __global__ void __launch_bounds__(128) few_kernel(const AttnArgs a) {
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const float r = row_pow2(amax);
-        qf[mt] = a.scale_log2 / r;
-        if (warp == (mt & 3)) {
+        if (t == 0) sm.qf[mt * 8 + g] = a.scale_log2 * inv_pow2(r);
 #pragma unroll
-            for (int i = 0; i < KC; ++i)
+        for (int i = 0; i < KC; ++i)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {   // word w of the 16-byte load: dims 4 w .. 4 w + 3 of the chunk
-                    const float *x = &v[i][w >> 1][(w & 1) * 4];
-                    uint4 f;
-                    split2(x[0] * r, x[1] * r, f.x, f.y);
-                    split2(x[2] * r, x[3] * r, f.z, f.w);
-                    sm.q[mt][i * 4 + w][lane] = f;
-                }
-        }
+            for (int w = 0; w < 4; ++w) {   // word w of the 16-byte load: dims 4 w .. 4 w + 3 of the chunk
+                const float *x = &v[i][w >> 1][(w & 1) * 4];
+                uint32_t h0, l0, h1, l1;
+                split2(x[0] * r, x[1] * r, h0, l0);
+                split2(x[2] * r, x[3] * r, h1, l1);
+                uint32_t *q = sm.q[mt][i * 4 + w][lane];
+                q[0] = h0;
+                q[1] = h1;
+                if (TWO) { q[FewSmem<T, D, MT>::QW - 2] = l0; q[FewSmem<T, D, MT>::QW - 1] = l1; }
+            }
     }
     __syncthreads();
 
-    float o[MT][NJ][2];
-    float m_run[MT], l_run[MT];
-    int tq[MT];                           // token row of this lane's query row
+    float o[MT][NJ][4];                   // dims 2 j, 2 j + 1 of the lane group's, rows 2 t, 2 t + 1: (d, r), (d, r'), (d', r), (d', r')
+    float mref[MT][2], l[MT][2], E[MT][2], qf[MT][2];
+    int tq[MT][2];                        // token row of this lane's query rows
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m_run[mt] = -INFINITY;
-        l_run[mt] = 0.0f;
-        const int m = m0 + mt * 8 + g;
-        tq[mt] = m < M ? t_first + m / G : INT_MIN / 2;   // a row of the tile's end: its results are not stored
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = 0.0f;
-    }
-    const int *trow = a.table + (size_t)s * a.stride;
-    const int end = min(list.n, (piece + 1) * a.chunk);
-    int at = piece * a.chunk + warp;
-
-    uint4 kr[2][KC];
-    uint32_t vr[4][VB / 4];
-    float ks = 0.0f, vs = 0.0f;
-    bool have = false;
-    auto load = [&](int i) {              // page i of the list -> registers
-        have = false;
-        if (i >= end) return;
-        const int page = trow[list.at(i)];
-        if (!a.p.has(page)) {
-            if (lane == 0) set_status(CT_STATUS_BAD_ARG);
-            return;                       // its rows count as not there
+        for (int e = 0; e < 2; ++e) {
+            const int m = m0 + mt * 8 + 2 * t + e;
+            mref[mt][e] = -INFINITY;
+            l[mt][e] = 0.0f;
+            E[mt][e] = 1.1754944e-38f;
+            qf[mt][e] = sm.qf[mt * 8 + 2 * t + e];
+            tq[mt][e] = t_first + min(m, M - 1) / G;
         }
-        have = true;
-        const size_t bk = a.p.block(page, a.layer, 0, hk), bv = bk + a.p.heads;
-        const uint8_t *kp = a.p.codes + bk * (ROWS * D), *vp = a.p.codes + bv * (ROWS * D);
-        ks = a.p.scales[bk];
-        vs = a.p.scales[bv];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.0f;
+    }
+    uint32_t loads = 0;                   // copies into each stage so far, modulo 2 (bit per stage)
+    for (int it = 0; it < mine; it += 2) {
+        bool there[2];
+        int j0[2];
+        float kscale[2], vscale[2];
+        bool fail = false;
 #pragma unroll
-            for (int c = 0; c < KC; ++c)
-                kr[n][c] = *reinterpret_cast<const uint4 *>(kp + (n * 8 + g) * D + (t + 4 * c) * 16);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint8_t *src = vp + (2 * t + (r & 1) + (r >> 1) * 8) * D + g * VB;
-            if (VB == 16) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(src);
-                vr[r][0] = x.x; vr[r][1] = x.y; vr[r][VB / 4 - 2] = x.z; vr[r][VB / 4 - 1] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                vr[r][0] = x.x; vr[r][1] = x.y;
+        for (int n = 0; n < 2; ++n) {
+            const int i = it + n, st = i % FEW_STAGES;
+            kscale[n] = __shfl_sync(0xffffffffu, ks, i & 31);
+            vscale[n] = __shfl_sync(0xffffffffu, vs, i & 31);
+            there[n] = i < mine && __shfl_sync(0xffffffffu, page, i & 31) >= 0;
+            j0[n] = list.at(e0 + 4 * i) * ROWS;
+            if (there[n] && !fail) {
+                fail = !__all_sync(0xffffffffu, mbar_wait(&sm.full[warp][st], (loads >> st) & 1, CT_STATUS_TIMEOUT_TMA));
+                loads ^= 1u << st;
             }
         }
-    };
-    load(at);
-    for (; at < end; at += 4) {
-        const int j0 = list.at(at) * ROWS;
-        const bool ok = have;
-        uint4 k[2][KC];
-        uint32_t v[4][VB / 4];
-        const float kscale = ks, vscale = vs;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int c = 0; c < KC; ++c) k[n][c] = kr[n][c];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int w = 0; w < VB / 4; ++w) v[r][w] = vr[r][w];
-        load(at + 4);
-        if (!ok) continue;
-        // every row of the tile sees the whole page
-        const bool whole = j0 + ROWS <= len && (!a.causal || j0 + ROWS - 1 <= t_lo) &&
-                           (!a.window || j0 > t_hi - a.window || j0 + ROWS <= a.sinks);
-        if (j0 + ROWS > len) {            // rows behind the last one may hold anything
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (j0 + 2 * t + (r & 1) + (r >> 1) * 8 >= len)
-#pragma unroll
-                    for (int w = 0; w < VB / 4; ++w) v[r][w] = 0;
+        if (fail) {                       // give the copies in flight once more the time to land, and stop
+            for (int x = it; x < min(it + FEW_STAGES, mine); ++x)
+                mbar_wait_for(&sm.full[warp][x % FEW_STAGES], (loads >> (x % FEW_STAGES)) & 1, CT_STATUS_TIMEOUT_TMA, CT_WAIT_NS / 4);
+            break;
         }
+        // S^T of both pages (one that is not there goes through with whatever its stage holds, unseen)
         float c[MT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int n = 0; n < 2; ++n) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) c[mt][n][0] = c[mt][n][1] = c[mt][n][2] = c[mt][n][3] = 0.0f;
+            for (int mt = 0; mt < MT; ++mt) c[mt][n][0] = c[mt][n][1] = c[mt][n][2] = c[mt][n][3] = 0.0f;
+            const uint8_t *kp = sm.kv[warp][(it + n) % FEW_STAGES][0];
+            uint4 k[2][KC];
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            uint32_t b[2][2];
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const uint4 &x = k[n][i / 4];
-                const uint32_t w = (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
-                codes4_to_half<FMT>(w, b[n][0], b[n][1]);
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const uint4 f = sm.q[mt][i][lane];
-                const uint32_t qa[4] = {f.x, f.y, f.z, f.w};
-                mma_f16(c[mt][0], qa, b[0][0], b[0][1]);
-                mma_f16(c[mt][1], qa, b[1][0], b[1][1]);
-            }
-        }
-        uint32_t pa[MT][4];
-        float rvs[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float f = qf[mt] * kscale;
-            float x[4];                   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-            bool any = true;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (c[mt][e >> 1][e & 1] + c[mt][e >> 1][2 + (e & 1)]) * f;
-            if (!whole) {
-                any = false;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool see = sees(a, tq[mt], j0 + 2 * t + (e & 1) + (e >> 1) * 8, len);
-                    if (!see) x[e] = -INFINITY;
-                    any |= see;
+                for (int i = 0; i < KC; ++i) {
+                    const int row = r * 8 + g;
+                    k[r][i] = *reinterpret_cast<const uint4 *>(kp + row * D + (((KC * t + i) ^ swz<D>(row)) << 4));
                 }
-                any |= __shfl_xor_sync(0xffffffffu, (int)any, 1) != 0;
-                any |= __shfl_xor_sync(0xffffffffu, (int)any, 2) != 0;
-            }
-            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m_run[mt], mx);
-            const float ref = mn == -INFINITY ? 0.0f : mn;
-            // probabilities times 2^14: the low fp16 parts stay normal numbers
-            float pr[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pr[e] = ex2(x[e] - ref + 14.0f);
-            split2(pr[0], pr[1], pa[mt][0], pa[mt][1]);
-            split2(pr[2], pr[3], pa[mt][2], pa[mt][3]);
-            const float corr = ex2(m_run[mt] - ref);   // 0 on the first page
-            l_run[mt] = l_run[mt] * corr + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
-            if (__any_sync(0xffffffffu, mn != m_run[mt])) {
+            for (int i = 0; i < KS; ++i) {
+                uint32_t ka[4];
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) { o[mt][j][0] *= corr; o[mt][j][1] *= corr; }
-            }
-            m_run[mt] = mn;
-            rvs[mt] = any ? vscale : 0.0f;   // a block that a row does not see adds nothing, whatever its scale
-        }
-#pragma unroll
-        for (int w = 0; w < VB / 4; ++w) {
-            // 4 dims of keys (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) as pairs over the key
-            uint32_t b[4][2];
-#pragma unroll
-            for (int hp = 0; hp < 2; ++hp) {
-                const uint32_t x = v[2 * hp][w], y = v[2 * hp + 1][w];
-                codes4_to_half<FMT>(__byte_perm(x, y, 0x5140), b[0][hp], b[1][hp]);
-                codes4_to_half<FMT>(__byte_perm(x, y, 0x7362), b[2][hp], b[3][hp]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
+                for (int r = 0; r < 2; ++r) {
+                    const uint4 &x = k[r][i / 4];
+                    const uint32_t w = (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
+                    codes4_to_half<FMT>(w, ka[r], ka[2 + r]);
+                }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16(d, pa[mt], b[e][0], b[e][1]);
-                    const int j = w * 4 + e;
-                    o[mt][j][0] = fmaf(rvs[mt], d[0] + d[2], o[mt][j][0]);
-                    o[mt][j][1] = fmaf(rvs[mt], d[1] + d[3], o[mt][j][1]);
+                    const uint32_t *q = sm.q[mt][i][lane];
+                    if (TWO) {
+                        const uint4 f = *reinterpret_cast<const uint4 *>(q);
+                        mma_f16(c[mt][n], ka, f.x, f.y);
+                        mma_f16(c[mt][n], ka, f.z, f.w);
+                    } else {
+                        const uint2 f = *reinterpret_cast<const uint2 *>(q);
+                        mma_f16(c[mt][n], ka, f.x, f.y);
+                    }
                 }
+            }
         }
+        // every row of the tile sees all of both pages
+        bool all_whole = true;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            all_whole = all_whole && there[n] && j0[n] + ROWS <= len && (!a.causal || j0[n] + ROWS - 1 <= t_lo) &&
+                        (!a.window || j0[n] > t_hi - a.window || j0[n] + ROWS <= a.sinks);
+        // probabilities
+        uint32_t ph[MT][2][2], pl[MT][2][2];   // B fragments of P.V: keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of row g
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            uint32_t see = 0xFFu;         // bit 4 n + e: (key g, row 2 t), (g, 2 t + 1), (g + 8, 2 t), (g + 8, 2 t + 1) of page n
+            float mx[2] = {-INFINITY, -INFINITY}, vm[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[mt][n][e] *= qf[mt][e & 1] * kscale[n];
+            if (all_whole) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    mx[e] = fmaxf(fmaxf(c[mt][0][e], c[mt][0][2 + e]), fmaxf(c[mt][1][e], c[mt][1][2 + e]));
+                    vm[e] = fmaxf(vscale[0], vscale[1]);
+                }
+            } else {
+                vm[0] = vm[1] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool y = there[n] && sees(a, tq[mt][e & 1], j0[n] + g + (e >> 1) * 8, len);
+                        if (y) mx[e & 1] = fmaxf(mx[e & 1], c[mt][n][e]);
+                        else see &= ~(1u << (4 * n + e));
+                        // some lane of the row sees a key of this page
+                        if (__ballot_sync(0xffffffffu, y) & (0x11111111u << t)) vm[e & 1] = fmaxf(vm[e & 1], vscale[n]);
+                    }
+            }
+            if (__any_sync(0xffffffffu, mx[0] > mref[mt][0] + THR || mx[1] > mref[mt][1] + THR ||
+                                            vm[0] > 16.0f * E[mt][0] || vm[1] > 16.0f * E[mt][1])) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+                    const bool move = mx[e] > mref[mt][e] + THR;
+                    const float mn = move ? mx[e] : mref[mt][e];
+                    const float En = vm[e] > 16.0f * E[mt][e] ? o_unit(vm[e]) : E[mt][e];
+                    const float cl = move ? ex2(mref[mt][e] - mn) : 1.0f, co = cl * (E[mt][e] * inv_pow2(En));
+                    l[mt][e] *= cl;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) { o[mt][j][e] *= co; o[mt][j][2 + e] *= co; }
+                    mref[mt][e] = mn;
+                    E[mt][e] = En;
+                }
+            }
+            float p[2][4], sub[2], vr[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sub[e] = OFF - (mref[mt][e] == -INFINITY ? 0.0f : mref[mt][e]);
+                vr[e] = inv_pow2(E[mt][e]);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[n][e] = ex2(c[mt][n][e] + sub[e & 1]);
+            if (!all_whole) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(see >> (4 * n + e) & 1)) p[n][e] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) l[mt][e] += (p[0][e] + p[0][2 + e]) + (p[1][e] + p[1][2 + e]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[n][e] *= vscale[n] * vr[e & 1];
+            if (!all_whole) {             // a block that a row does not see adds nothing, whatever its scale
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(see >> (4 * n + e) & 1)) p[n][e] = 0.0f;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t hi, lo;
+                    if (TWO) {
+                        split2(p[n][2 * h], p[n][2 * h + 1], hi, lo);
+                        pl[mt][n][h] = transpose8(lo);
+                    } else {
+                        const __half2 x = __floats2half2_rn(p[n][2 * h], p[n][2 * h + 1]);
+                        hi = *reinterpret_cast<const uint32_t *>(&x);
+                    }
+                    ph[mt][n][h] = transpose8(hi);
+                }
+            }
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const uint8_t *vp = sm.kv[warp][(it + n) % FEW_STAGES][1];
+            uint32_t v[4][VB / 4];        // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 2 * t + (r & 1) + (r >> 1) * 8;
+                if (VB == 16) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(vp + row * D + ((g ^ swz<D>(row)) << 4));
+                    v[r][0] = x.x; v[r][1] = x.y; v[r][VB / 4 - 2] = x.z; v[r][VB / 4 - 1] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(vp + row * D + (((g >> 1) ^ swz<D>(row)) << 4) + (g & 1) * 8);
+                    v[r][0] = x.x; v[r][1] = x.y;
+                }
+            }
+            if (!all_whole && (!there[n] || j0[n] + ROWS > len)) {   // what is not a row may hold anything
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!there[n] || j0[n] + 2 * t + (r & 1) + (r >> 1) * 8 >= len)
+#pragma unroll
+                        for (int w = 0; w < VB / 4; ++w) v[r][w] = 0;
+            }
+#pragma unroll
+            for (int w = 0; w < VB / 4; ++w) {
+                uint32_t x[2][4];         // [key pair][dim of the word]: codes of two keys of one dim as fp16
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    codes4_to_half<FMT>(__byte_perm(v[2 * h][w], v[2 * h + 1][w], 0x5140), x[h][0], x[h][1]);
+                    codes4_to_half<FMT>(__byte_perm(v[2 * h][w], v[2 * h + 1][w], 0x7362), x[h][2], x[h][3]);
+                }
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const uint32_t va[4] = {x[0][2 * d], x[0][2 * d + 1], x[1][2 * d], x[1][2 * d + 1]};
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        mma_f16(o[mt][w * 2 + d], va, ph[mt][n][0], ph[mt][n][1]);
+                        if (TWO) mma_f16(o[mt][w * 2 + d], va, pl[mt][n][0], pl[mt][n][1]);
+                    }
+                }
+            }
+        }
+        __syncwarp();                     // the stages are read
+        issue(it + FEW_STAGES);
+        issue(it + FEW_STAGES + 1);
     }
 
     // ---- the four warps' results -> one
-    __syncthreads();                      // the queries' fragments are read
+    __syncthreads();                      // every warp has read its last stage
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        float l = l_run[mt];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) { sm.m[warp][mt * 8 + g] = m_run[mt]; sm.l[warp][mt * 8 + g] = l; }
-        float *dst = sm.o[warp][mt * 8 + g];
-        // columns 2 t, 2 t + 1 of tile j: dims (2 t) * VB + j, (2 t + 1) * VB + j
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e) {
+            float x = l[mt][e];
 #pragma unroll
-            for (int j = 0; j < NJ; j += 4)
-                *reinterpret_cast<float4 *>(dst + (2 * t + e) * VB + j) =
-                    make_float4(o[mt][j][e], o[mt][j + 1][e], o[mt][j + 2][e], o[mt][j + 3][e]);
-    }
+            for (int y = 4; y < 32; y *= 2) x += __shfl_xor_sync(0xffffffffu, x, y);
+            const int row = mt * 8 + 2 * t + e;
+            if (g == 0) { sm.m[warp][row] = mref[mt][e]; sm.l[warp][row] = x; }
+            float *dst = sm.o[warp][row] + g * VB;
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2)
+                *reinterpret_cast<float4 *>(dst + 2 * j) =
+                    make_float4(o[mt][j][e] * E[mt][e], o[mt][j][2 + e] * E[mt][e], o[mt][j + 1][e] * E[mt][e],
+                                o[mt][j + 1][2 + e] * E[mt][e]);
+        }
     __syncthreads();
     const size_t rows_all = (size_t)a.n_rows * a.heads;
     for (int i = threadIdx.x; i < 8 * MT * (D / 4); i += 128) {
@@ -369,25 +506,25 @@ __global__ void __launch_bounds__(128) few_kernel(const AttnArgs a) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm.m[w][row]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
-        float l = 0.0f;
+        float lsum = 0.0f;
         float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float f = ex2(sm.m[w][row] - ref);
-            l += sm.l[w][row] * f;
+            lsum += sm.l[w][row] * f;
             const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][row][d]);
             acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
         }
         const size_t r = (size_t)sp.first + m / G;
         const int h = hk * G + m % G;
         if (pieces == 1) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing: zeros
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;   // a row that sees nothing: zeros
             store4(static_cast<T *>(a.out) + r * a.ldo + (size_t)h * D + d, acc.x * inv, acc.y * inv, acc.z * inv,
                    acc.w * inv);
         } else {
             const size_t b = (r * a.heads + h) * a.max_chunks + piece;
             *reinterpret_cast<float4 *>(a.part + b * D + d) = acc;
-            if (d == 0) *reinterpret_cast<float2 *>(a.part + rows_all * a.max_chunks * D + b * 2) = make_float2(mx, l);
+            if (d == 0) *reinterpret_cast<float2 *>(a.part + rows_all * a.max_chunks * D + b * 2) = make_float2(mx, lsum);
         }
     }
 }

@@ -33,20 +33,16 @@ class KV8Error(RuntimeError):
         self.code = code
 
 
-def _check(rc, name):
-    if rc != 0:
-        raise KV8Error(name, rc)
-
-
 def _need(cond, what):
     if not cond:
         raise ValueError(what)
 
 
 def _ints(t, shape, device, what):
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_contiguous() and t.device == device
-          and (shape is None or tuple(t.shape) == shape), f"{what}: a contiguous int32 tensor"
-          + (f" {list(shape)}" if shape is not None else "") + f" on {device}")
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_contiguous() and t.device == device
+            and (shape is None or t.shape == shape)):
+        raise ValueError(f"{what}: a contiguous int32 tensor" + (f" {list(shape)}" if shape is not None else "")
+                         + f" on {device}")
     return t.data_ptr()
 
 
@@ -59,6 +55,7 @@ class Seqs:
         q = _ints(lens, (table.shape[0],), table.device, "lens")
         self.table, self.lens = table, lens
         self.n, self.max_pages = table.shape
+        self.device = table.device
         self.c = abi.KV8Seqs(p, q, self.n, self.max_pages)
         self.ref = ctypes.addressof(self.c)
 
@@ -82,6 +79,7 @@ class Cache:
         self.codes, self.scales, self.refs, self.fmt = codes, scales, refs, fmt
         self.n_pages, self.n_layers, _, self.kv_heads, _, self.head_dim = codes.shape
         self.device = codes.device
+        self.scale = self.head_dim ** -0.5
         r = _ints(refs, (self.n_pages,), self.device, "refs") if refs is not None else None
         self.lib = abi.load()
         self.c = abi.KV8Cache(codes.data_ptr(), scales.data_ptr(), r, self.n_pages, self.n_layers, self.kv_heads,
@@ -94,42 +92,52 @@ class Cache:
         return cls(torch.zeros(*shape, ROWS, head_dim, dtype=torch.uint8, device=device),
                    torch.zeros(*shape, device=device), torch.zeros(n_pages, dtype=torch.int32, device=device), fmt)
 
-    # ---- helpers
+    # ---- helpers (short paths: a decode step's calls are a few microseconds of GPU work each)
     def _call(self, name, *args):
         """The C call with this device current, on its current torch stream."""
-        if torch.cuda.current_device() == self.device.index:
-            rc = getattr(self.lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+        index = self.device.index
+        if torch._C._cuda_getDevice() == index:
+            rc = getattr(self.lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
-            with torch.cuda.device(self.device):
-                rc = getattr(self.lib, name)(*args, torch.cuda.current_stream().cuda_stream)
-        _check(rc, name)
+            with torch.cuda.device(index):
+                rc = getattr(self.lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            raise KV8Error(name, rc)
 
     def _seqs(self, s):
-        _need(s.table.device == self.device, f"the sequences are not on {self.device}")
+        if s.device != self.device:
+            raise ValueError(f"the sequences are not on {self.device}")
         return s.ref
 
     def _layer(self, layer):
-        _need(0 <= layer < self.n_layers, f"layer: 0 .. {self.n_layers - 1}")
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer: 0 .. {self.n_layers - 1}")
         return layer
 
-    def _rows(self, x, heads, what):
-        """Row stride of [rows, heads, head_dim] with each row contiguous."""
-        _need(x.dim() == 3 and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads)
-              and x.shape[0] > 0 and x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == self.head_dim)
-              and x.dtype in _TYPES and x.device == self.device,
-              f"{what}: float32 or bfloat16 [rows, {heads or 'heads'}, {self.head_dim}] on {self.device}, rows contiguous")
-        ld = x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
-        _need(ld >= x.shape[1] * x.shape[2] and ld * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0,
-              f"{what}: rows of 16-byte alignment that do not overlap")
-        return ld
+    def _rows(self, x, what):
+        """Rows, heads and row stride of [rows, heads, head_dim] with each row contiguous, and its address."""
+        try:
+            (n, h, d), (ld, sh, sd) = x.shape, x.stride()
+        except (ValueError, AttributeError):
+            raise ValueError(f"{what}: [rows, heads, {self.head_dim}]") from None
+        if n == 1:
+            ld = h * d
+        p = x.data_ptr()
+        if (d != self.head_dim or n == 0 or h == 0 or sd != 1 or (sh != d and h > 1) or ld < h * d
+                or x.dtype not in _TYPES or x.device != self.device or (p | ld * x.element_size()) & 15):
+            raise ValueError(f"{what}: float32 or bfloat16 [rows, heads, {self.head_dim}] on {self.device}, each row "
+                             "contiguous, rows of 16-byte alignment that do not overlap")
+        return n, h, ld, p
 
     def _ws(self, ws, need):
-        if need == 0:
-            return None, None, 0
+        """Address and size of a workspace: the caller's (the C call checks its size) or a new one of need() bytes."""
         if ws is None:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        _need(ws.dtype == torch.uint8 and ws.is_contiguous() and ws.device == self.device and ws.numel() >= need,
-              f"ws: a contiguous uint8 tensor of at least {need} bytes on {self.device}")
+            n = need()
+            if n == 0:
+                return None, None, 0
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        elif ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != self.device:
+            raise ValueError(f"ws: a contiguous uint8 tensor on {self.device}")
         return ws, ws.data_ptr(), ws.numel()
 
     def _starts(self, seqs, rows, row_start, max_rows):
@@ -141,40 +149,43 @@ class Cache:
     # ---- operators
     def append(self, layer, seqs, k, v, row_start=None, max_rows=1):
         """Write the rows k, v [rows, kv_heads, head_dim] (ct_kv8_append)."""
-        ldk, ldv = self._rows(k, self.kv_heads, "k"), self._rows(v, self.kv_heads, "v")
-        _need(k.dtype == v.dtype and k.shape == v.shape, "k and v: the same shape and type")
-        rs = self._starts(seqs, k.shape[0], row_start, max_rows)
-        self._call("ct_kv8_append", self.ref, self._layer(layer), self._seqs(seqs), k.data_ptr(), ldk, v.data_ptr(),
-                   ldv, _TYPES[k.dtype], rs, max_rows)
-
-    def _attend_ws_bytes(self, seqs, q, max_rows, max_len, causal, window, sinks):
-        return self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, _TYPES[q.dtype], q.shape[0], max_rows, max_len,
-                                             q.shape[1], int(causal), window, sinks)
+        n, h, ldk, pk = self._rows(k, "k")
+        nv, hv, ldv, pv = self._rows(v, "v")
+        _need(k.dtype == v.dtype and n == nv and h == hv == self.kv_heads,
+              f"k and v: the same type and number of rows, {self.kv_heads} heads")
+        rs = self._starts(seqs, n, row_start, max_rows)
+        self._call("ct_kv8_append", self.ref, self._layer(layer), self._seqs(seqs), pk, ldk, pv, ldv,
+                   _TYPES[k.dtype], n, rs, max_rows)
 
     def attend_workspace(self, seqs, q, max_rows=1, max_len=None, causal=True, window=0, sinks=0):
         """A workspace for `attend` calls of these sizes (one per stream that may run them at the same time)."""
-        self._rows(q, None, "q")
-        n = self._attend_ws_bytes(seqs, q, max_rows, seqs.max_pages * ROWS if max_len is None else max_len, causal,
-                                  window, sinks)
+        n, h, _, _ = self._rows(q, "q")
+        n = self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, _TYPES[q.dtype], n, max_rows,
+                                          seqs.max_pages * ROWS if max_len is None else max_len, h, int(causal),
+                                          window, sinks)
         return torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
 
     def attend(self, layer, seqs, q, out=None, row_start=None, max_rows=1, max_len=None, causal=True, window=0,
                sinks=0, scale=None, ws=None):
         """Attention of q [rows, heads, head_dim] over the sequences' pages (ct_kv8_attn); max_len bounds their
         lengths (default: the table's width)."""
-        ldq = self._rows(q, None, "q")
+        n, h, ldq, pq = self._rows(q, "q")
+        typ = _TYPES[q.dtype]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        ldo = self._rows(out, q.shape[1], "out")
-        _need(out.dtype == q.dtype and out.shape == q.shape, "out: q's shape and type")
-        _need(q.shape[1] % self.kv_heads == 0, "heads: a multiple of kv_heads")
-        rs = self._starts(seqs, q.shape[0], row_start, max_rows)
-        max_len = seqs.max_pages * ROWS if max_len is None else max_len
-        need = self._attend_ws_bytes(seqs, q, max_rows, max_len, causal, window, sinks)
-        ws, p, n = self._ws(ws, need)
-        self._call("ct_kv8_attn", self.ref, self._layer(layer), self._seqs(seqs), q.data_ptr(), ldq, out.data_ptr(),
-                   ldo, _TYPES[q.dtype], q.shape[0], rs, max_rows, max_len, q.shape[1],
-                   self.head_dim ** -0.5 if scale is None else scale, int(causal), window, sinks, p, n)
+            out = torch.empty((n, h, self.head_dim), dtype=q.dtype, device=self.device)
+            ldo, po = h * self.head_dim, out.data_ptr()
+        else:
+            no, ho, ldo, po = self._rows(out, "out")
+            _need(out.dtype == q.dtype and no == n and ho == h, "out: q's shape and type")
+        _need(h % self.kv_heads == 0, "heads: a multiple of kv_heads")
+        rs = self._starts(seqs, n, row_start, max_rows)
+        if max_len is None:
+            max_len = seqs.max_pages * ROWS
+        causal = int(causal)
+        ws, pw, nw = self._ws(ws, lambda: self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, typ, n, max_rows, max_len,
+                                                                       h, causal, window, sinks))
+        self._call("ct_kv8_attn", self.ref, self._layer(layer), self._seqs(seqs), pq, ldq, po, ldo, typ, n, rs,
+                   max_rows, max_len, h, self.scale if scale is None else scale, causal, window, sinks, pw, nw)
         return out
 
     def pages_workspace(self, seqs):
@@ -183,7 +194,7 @@ class Cache:
         return torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
 
     def _pages_ws(self, seqs, ws):
-        return self._ws(ws, self.lib.ct_kv8_pages_ws_bytes(self.ref, seqs.n))
+        return self._ws(ws, lambda: self.lib.ct_kv8_pages_ws_bytes(self.ref, seqs.n))
 
     def reserve(self, seqs, add, ws=None):
         """lens += add, with pages for the new rows (ct_kv8_reserve)."""

@@ -75,11 +75,12 @@ typedef struct {
 } ct_kv8_seqs;
 
 /* Write the K and V rows of this call into `layer`.
- * k, v: [rows][kv_heads * head_dim] of `type`, row strides ldk / ldv in
+ * k, v: [n_rows][kv_heads * head_dim] of `type`, row strides ldk / ldv in
  * elements; 16-byte aligned, strides a multiple of 16 bytes.  Sequence s owns
  * rows row_start[s] .. row_start[s + 1] - 1, at most max_rows of them;
  * row_start NULL means row s for each sequence (a decode step; max_rows = 1),
- * and none for a sequence of length 0.  len[s] already counts them: they are token rows len[s] - n .. len[s] - 1.
+ * and none for a sequence of length 0.  len[s] already counts the rows: they are
+ * token rows len[s] - n .. len[s] - 1.
  *
  * Each block takes the smallest power of two as its scale that brings its
  * largest finite magnitude within the codes' range; a block that already held
@@ -93,7 +94,7 @@ typedef struct {
  * (status): two sequences may share full pages only, as ct_kv8_fork
  * leaves them.  max_rows up to 1 << 20. */
 int ct_kv8_append(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const void *k, int ldk, const void *v,
-                  int ldv, int type, const int *row_start, int max_rows, void *stream);
+                  int ldv, int type, int n_rows, const int *row_start, int max_rows, void *stream);
 
 /* out[r][h] = softmax_j(scale * q[r][h] . K[j][h / g]) V[j][h / g], g = heads / kv_heads,
  * over the rows j of r's sequence that r sees.

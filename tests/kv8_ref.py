@@ -81,10 +81,11 @@ def sees(t, j, length, causal, window, sinks):
 
 
 def attend(cache, layer, table, lens, q, starts, heads_kv, scale, causal=True, window=0, sinks=0):
-    """out, mass = sum p |v|, and reach = max_j scale max|q| sum_d |k|: what a row's rounding errors scale with."""
+    """out, mass = sum p |v|, reach = max_j scale max|q| sum_d |k| and total = sum |v|: what a row's rounding errors
+    scale with."""
     R, H, D = q.shape
     G = H // heads_kv
-    out, mass, reach = np.zeros((R, H, D)), np.zeros((R, H, D)), np.zeros((R, H, 1))
+    out, mass, total, reach = np.zeros((R, H, D)), np.zeros((R, H, D)), np.zeros((R, H, D)), np.zeros((R, H, 1))
     for s in range(len(lens)):
         n, L = starts[s + 1] - starts[s], max(int(lens[s]), 0)
         if not L:
@@ -108,10 +109,11 @@ def attend(cache, layer, table, lens, q, starts, heads_kv, scale, causal=True, w
                 j = see[i]
                 out[r.start + i, h] = p[i, j] @ V[j]
                 mass[r.start + i, h] = p[i, j] @ np.abs(V[j])
+                total[r.start + i, h] = np.abs(V[j]).sum(0)
             qm = np.abs(q[r, h].astype(np.float64)).max(1)
             k1 = np.abs(K).sum(1)
             reach[r, h, 0] = scale * qm * np.max(np.where(see, k1[None], 0.0), 1)
-    return out, mass, reach
+    return out, mass, reach, total
 
 
 # ---- pages

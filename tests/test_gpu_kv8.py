@@ -9,7 +9,9 @@ Attention tolerances, derived per output from the kernels' arithmetic.  With rea
   steps) + 2^-20 for the exponential, so a probability is off by twice that, relative;
   probabilities as two fp16 add 2^-22, the sums over n pages (n + 64) 2^-22 (in calls of many bf16 rows the
   probability is one fp16: 2^-11 instead);
-  all of it scales with mass; rounding the result to its type adds half a step, |out| eps / 2.
+  an fp16 has an absolute step below its normal numbers: a probability's error is at least 2^-32 of the row's largest
+  (2^-28 as one fp16), whatever its own size, which adds that times the sum of |v|;
+  all the rest of it scales with mass; rounding the result to its type adds half a step, |out| eps / 2.
 """
 import importlib
 import math
@@ -185,11 +187,11 @@ def test_append_leaves_out_what_it_cannot_write(kv8, torch):
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------
-def tolerance(out, mass, reach, dim, pages, typ, single):
+def tolerance(out, mass, reach, total, dim, pages, typ, single):
     import torch
     dx = reach * (dim / 16 + 10) * 2.0 ** -22 + 2.0 ** -20
     rel = 2.2 * dx + (2.0 ** -11 if single else 2.0 ** -22) + (pages + 64) * 2.0 ** -22
-    return mass * rel + np.abs(out) * (torch.finfo(getattr(torch, typ)).eps / 2) + 1e-30
+    return mass * rel + total * 2.0 ** (-28 if single else -32) + np.abs(out) * (torch.finfo(getattr(torch, typ)).eps / 2) + 1e-30
 
 
 def check_attend(kv8, c, s, rc, table, lens, rows, heads, typ, seed=1, causal=True, window=0, sinks=0, scale=None,
@@ -208,10 +210,10 @@ def check_attend(kv8, c, s, rc, table, lens, rows, heads, typ, seed=1, causal=Tr
     got = c.attend(layer, s, q, out=out, **kw)
     assert got is out and c.status() == 0
     assert bool((out[n:] == 7.0).all())          # rows behind the last sequence
-    want, mass, reach = ref.attend(rc, layer, table, lens, q[:n].float().cpu().numpy(), st, c.kv_heads, scale, causal,
+    want, mass, reach, total = ref.attend(rc, layer, table, lens, q[:n].float().cpu().numpy(), st, c.kv_heads, scale, causal,
                                    window, sinks)
     o = out[:n].float().cpu().numpy().astype(np.float64)
-    tol = tolerance(want, mass, reach, D, max(len(r) for r in table), typ, typ == "bfloat16")
+    tol = tolerance(want, mass, reach, total, D, max(len(r) for r in table), typ, typ == "bfloat16")
     bad = ~(np.abs(o - want) <= tol)
     bad &= ~(np.isnan(o) & np.isnan(want))
     assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:5].tolist(), float(np.nanmax(np.abs(o - want) / tol)))
@@ -358,7 +360,7 @@ def test_attention_leaves_out_bad_sequences(kv8, torch):
     assert c.status() == BAD_ARG
     rc1 = ref.Cache(rc.v, rc.s, rc.refs, "int8")
     pages = [table[2][0], table[2][2]]
-    want, _, _ = ref.attend(rc1, 0, [pages], [24], q[2:].cpu().numpy(), [0, 1], 1, 0.125)
+    want, _, _, _ = ref.attend(rc1, 0, [pages], [24], q[2:].cpu().numpy(), [0, 1], 1, 0.125)
     assert np.allclose(got[2].cpu().numpy(), want[0], rtol=1e-4, atol=1e-5)
     st = dev([0, 1, 50, 3])                      # spans outside the packed rows
     out = torch.full_like(q, 7.0)
@@ -600,9 +602,9 @@ def test_beam_search_run(kv8, torch, fmt):
             c.append(layer, a, k, v, row_start=dev(st), max_rows=max(add))
             rc.append(layer, table, lens, k.cpu().numpy(), v.cpu().numpy(), st)
             o = c.attend(layer, a, q, row_start=dev(st), max_rows=max(add), window=window, sinks=sinks)
-            want, mass, reach = ref.attend(rc, layer, table, lens, q.cpu().numpy(), st, kvh, D ** -0.5, True, window, sinks)
+            want, mass, reach, total = ref.attend(rc, layer, table, lens, q.cpu().numpy(), st, kvh, D ** -0.5, True, window, sinks)
             got = o[:st[-1]].cpu().numpy()
-            assert (np.abs(got - want[:st[-1]]) <= tolerance(want, mass, reach, D, width, "float32", False)[:st[-1]]).all()
+            assert (np.abs(got - want[:st[-1]]) <= tolerance(want, mass, reach, total, D, width, "float32", False)[:st[-1]]).all()
         c.trim(a, window, sinks)
         ref.trim(table, lens, refs, window, sinks)
         parents = [g * beams + int(rng.integers(0, beams)) if step else g * beams for g in range(groups) for _ in range(beams)]

@@ -54,12 +54,12 @@ BAD_SEQS = [dict(len=None), dict(n_seqs=0), dict(n_seqs=65536), dict(table_strid
 
 
 def _append(lib, args, cache=None, seqs=None, **kw):
-    d = dict(layer=0, k=args.a, ldk=128, v=args.a, ldv=128, type=0, rs=args.a, max_rows=4)
+    d = dict(layer=0, k=args.a, ldk=128, v=args.a, ldv=128, type=0, n_rows=9, rs=args.a, max_rows=4)
     d.update(kw)
     c = args.cache() if cache is None else cache
     s = args.seqs() if seqs is None else seqs
     return lib.ct_kv8_append(ctypes.byref(c), d["layer"], ctypes.byref(s), d["k"], d["ldk"], d["v"], d["ldv"], d["type"],
-                             d["rs"], d["max_rows"], None)
+                             d["n_rows"], d["rs"], d["max_rows"], None)
 
 
 def _attn(lib, args, cache=None, seqs=None, **kw):
@@ -105,7 +105,8 @@ def test_bad_sequences_are_refused(lib, args, bad):
 
 @pytest.mark.parametrize("bad", [
     dict(layer=-1), dict(layer=2), dict(k=None), dict(v=None), dict(ldk=127), dict(ldv=126), dict(ldk=130),
-    dict(type=2), dict(max_rows=0), dict(max_rows=(1 << 20) + 1), dict(rs=None)], ids=str)
+    dict(type=2), dict(n_rows=0), dict(max_rows=0), dict(max_rows=(1 << 20) + 1), dict(rs=None),
+    dict(rs=None, max_rows=1, n_rows=2)], ids=str)
 def test_append_refuses(lib, args, bad):
     assert _append(lib, args, **bad) == CT_EINVAL
     assert _append(lib, args, k=args.a + 8) == CT_EINVAL
@@ -188,7 +189,7 @@ def test_reference_attention_of_one_key_is_its_value():
     c = ref.Cache(rng.integers(-127, 128, (2, 1, 2, 1, 16, 64)).astype(float), np.full((2, 1, 2, 1), 0.25),
                   np.ones(2, int), "int8")
     q = rng.standard_normal((2, 1, 64))
-    out, mass, _ = ref.attend(c, 0, [[1, 0]], [2], q, [0, 2], 1, 0.125)
+    out, mass, _, _ = ref.attend(c, 0, [[1, 0]], [2], q, [0, 2], 1, 0.125)
     assert np.allclose(out[0, 0], c.v[1, 0, 1, 0, 0] * 0.25) and np.allclose(mass[0], np.abs(out[0]))
-    out, _, _ = ref.attend(c, 0, [[1, 0]], [18], q, [0, 2], 1, 0.125, window=1, sinks=0)
+    out, _, _, _ = ref.attend(c, 0, [[1, 0]], [18], q, [0, 2], 1, 0.125, window=1, sinks=0)
     assert np.allclose(out[:, 0], c.v[0, 0, 1, 0, :2] * 0.25)
