@@ -13,7 +13,11 @@ namespace kv8 {
 // ---- rows -> blocks -------------------------------------------------------------
 // One warp per (sequence, touched page, kv head, K or V): it reads the block's
 // new rows once (16 bytes a lane, whole rows side by side), takes the largest
-// magnitude by shuffles, and writes codes from the same registers.
+// magnitude as the maximum of the bit patterns without their signs (magnitudes
+// order as unsigned integers, two bf16 at a time), and writes codes from the
+// same registers.  Blocks with an infinity or a NaN take a path of their own.
+// The loads hang together as length -> rows and page -> scale, so the rows are
+// under way before the page is known.
 struct AppendArgs {
     Pool p;
     const int *table, *len, *row_start;
@@ -39,41 +43,56 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
     const int p0 = sp.len - sp.n;
     const int blk = p0 / ROWS + item / (2 * a.p.heads);
     if (blk > (sp.len - 1) / ROWS) return;
-    const int page = a.table[(size_t)s * a.stride + blk];
-    if (!a.p.has(page) || (a.p.refs && a.p.refs[page] != 1)) {
-        if (lane == 0) set_status(CT_STATUS_BAD_ARG);
-        return;
-    }
     const int lo = max(p0 - blk * ROWS, 0), hi = min(sp.len - blk * ROWS, ROWS);   // the block's new rows
     const int rl = lane / LPR, c = (lane % LPR) * EPL;
     const T *src = static_cast<const T *>(a.src[kv]) +
                    ((size_t)sp.first + (blk * ROWS - p0)) * (size_t)a.ld[kv] + (size_t)h * D + c;
     uint4 x[PASSES];
-    float amax = 0.0f;
-    bool nan = false;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int r = i * RPP + rl;
         x[i] = make_uint4(0, 0, 0, 0);
         if (r >= lo && r < hi) x[i] = *reinterpret_cast<const uint4 *>(src + (ptrdiff_t)r * a.ld[kv]);
     }
+    const int page = a.table[(size_t)s * a.stride + blk];
+    const bool there = a.p.has(page);
+    const size_t b = a.p.block(there ? page : 0, a.layer, kv, h);
+    const int refs = a.p.refs && there ? a.p.refs[page] : 1;
+    const float old = lo > 0 ? a.p.scales[b] : 0.0f;
+    if (!there || refs != 1) {
+        if (lane == 0) set_status(CT_STATUS_BAD_ARG);
+        return;
+    }
+    uint32_t top = 0;                     // largest magnitude's bits
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-        const T *e = reinterpret_cast<const T *>(&x[i]);
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-            const float v = fabsf(to_f32(e[j]));
-            nan |= v != v;
-            if (v < INFINITY) amax = fmaxf(amax, v);
-        }
+        for (int j = 0; j < 4; ++j)
+            top = sizeof(T) == 2 ? __vmaxu2(top, w[j] & 0x7FFF7FFFu) : max(top, w[j] & 0x7FFFFFFFu);
     }
-    amax = warp_max(amax);
-    nan = __any_sync(0xffffffffu, nan);
-    const size_t b = a.p.block(page, a.layer, kv, h);
+    if (sizeof(T) == 2) top = max(top >> 16, top & 0xFFFFu) << 16;
+    top = __reduce_max_sync(0xffffffffu, top);
+    const bool special = top >= 0x7F800000u;   // an infinity or a NaN
+    bool nan = false;
+    if (special) {
+        float amax = 0.0f;                // of the finite ones
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const T *e = reinterpret_cast<const T *>(&x[i]);
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) {
+                const float v = fabsf(to_f32(e[j]));
+                nan |= v != v;
+                if (v < INFINITY) amax = fmaxf(amax, v);
+            }
+        }
+        top = __float_as_uint(warp_max(amax));
+        nan = __any_sync(0xffffffffu, nan);
+    }
     uint8_t *dst = a.p.codes + b * (ROWS * D) + c;
-    float scale = block_scale<FMT>(amax), shrink = 1.0f;
+    float scale = block_scale<FMT>(__uint_as_float(top)), shrink = 1.0f;
     if (lo > 0) {
-        const float old = a.p.scales[b];
         nan |= old != old;
         scale = fmaxf(scale, old);
         shrink = old / scale;
@@ -83,28 +102,30 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
     for (int i = 0; i < PASSES; ++i) {
         const int r = i * RPP + rl;
         uint32_t w[EPL / 4];
+        uint32_t *o = reinterpret_cast<uint32_t *>(dst + r * D);
         if (r >= lo && r < hi) {
             const T *e = reinterpret_cast<const T *>(&x[i]);
+            float y[EPL];
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                float y = to_f32(e[j]) * inv;
-                if (y != y) y = 0.0f;
-                const uint32_t code = f32_to_code<FMT>(y);
-                w[j / 4] = (j & 3) ? w[j / 4] | code << (8 * (j & 3)) : code;
+            for (int j = 0; j < EPL; ++j) y[j] = to_f32(e[j]) * inv;   // exact: scale is a power of two
+            if (special) {
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) y[j] = y[j] != y[j] ? 0.0f : fminf(fmaxf(y[j], -448.0f), 448.0f);
             }
-        } else if (r < lo && shrink < 1.0f) {   // rows that were there: rounded to the grown scale
-            const uint32_t *o = reinterpret_cast<const uint32_t *>(dst + r * D);
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                const uint32_t code = f32_to_code<FMT>(code_to_f32<FMT>((o[j / 4] >> (8 * (j & 3))) & 0xFFu) * shrink);
-                w[j / 4] = (j & 3) ? w[j / 4] | code << (8 * (j & 3)) : code;
+            for (int j = 0; j < EPL; j += 4) w[j / 4] = codes4<FMT>(y[j], y[j + 1], y[j + 2], y[j + 3], special);
+        } else if (r < lo && shrink < 1.0f) {   // rows that were there: rounded to the grown scale
+#pragma unroll
+            for (int j = 0; j < EPL; j += 4) {
+                const uint32_t u = o[j / 4];
+                w[j / 4] = codes4<FMT>(code_to_f32<FMT>(u & 0xFFu) * shrink, code_to_f32<FMT>(u >> 8 & 0xFFu) * shrink,
+                                       code_to_f32<FMT>(u >> 16 & 0xFFu) * shrink, code_to_f32<FMT>(u >> 24) * shrink, false);
             }
         } else {
             continue;
         }
-        uint32_t *o = reinterpret_cast<uint32_t *>(dst + r * D);
-#pragma unroll
-        for (int j = 0; j < EPL / 4; ++j) o[j] = w[j];
+        if (EPL == 8) *reinterpret_cast<uint2 *>(o) = make_uint2(w[0], w[EPL / 4 - 1]);
+        else *o = w[0];
     }
     __syncwarp();   // every lane has read the old scale
     if (lane == 0) a.p.scales[b] = nan ? __uint_as_float(0x7FC00000u) : scale;
@@ -546,7 +567,12 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
         while (chunk > 4 && ctas * ((list + chunk - 1) / chunk) < 592) chunk /= 2;
     } else {
         // whole key tiles; one piece once the tiles alone give every SM a CTA
-        const long long pieces = std::min(std::max(1ll, 148 / ctas), std::max(1ll, list / (4 * KB)));
+        long long pieces = std::min(std::max(1ll, 148 / ctas), std::max(1ll, list / (4 * KB)));
+        // The tensor core truncates each of its fp32 sums, so an error grows with the
+        // keys summed into one accumulator.  fp32 results take at most 2048 keys a
+        // piece (a sixteenth of them past 32,768) and join the pieces with rounded
+        // sums: against 64 bits 1.0e-6 instead of 2.1e-6 at 4000 keys.
+        if (type == CT_KV8_F32) pieces = std::max(pieces, std::min(16ll, (list + 127) / 128));
         chunk = ((list + pieces - 1) / pieces + KB - 1) / KB * KB;
     }
     pl.chunk = (int)chunk;

@@ -77,11 +77,25 @@ __device__ __forceinline__ float code_to_f32(uint32_t byte) {
     return (float)v;
 }
 
-// nearest code, ties to even, saturating; y is not NaN
+// Nearest codes of four values, ties to even, as one word.  E4M3 saturates.  int8:
+// adding 1.5 * 2^23 rounds to the integer that the sum's low byte then holds, for
+// magnitudes up to 127 (`clamp`: larger ones are cut to that first).
 template <int FMT>
-__device__ __forceinline__ uint32_t f32_to_code(float y) {
-    if (FMT == CT_KV8_INT8) return (uint32_t)__float2int_rn(fminf(fmaxf(y, -127.0f), 127.0f)) & 0xFFu;
-    return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, bool clamp) {
+    if (FMT == CT_KV8_E4M3) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        return lo | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+    }
+    if (clamp) {
+        a = fminf(fmaxf(a, -127.0f), 127.0f);
+        b = fminf(fmaxf(b, -127.0f), 127.0f);
+        c = fminf(fmaxf(c, -127.0f), 127.0f);
+        d = fminf(fmaxf(d, -127.0f), 127.0f);
+    }
+    constexpr float magic = 12582912.0f;
+    const uint32_t ab = __byte_perm(__float_as_uint(a + magic), __float_as_uint(b + magic), 0x0040);
+    const uint32_t cd = __byte_perm(__float_as_uint(c + magic), __float_as_uint(d + magic), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
 }
 
 // The smallest power of two that brings amax (finite, >= 0) within the codes'

@@ -218,11 +218,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                     tc_fence_after();
                     const uint64_t vd = sw128_mn_desc(smem_u32(sm.kv[n & 3][0]));
 #pragma unroll
-                    for (int p = 0; p < (TWO ? 2 : 1); ++p)
+                    for (int p = TWO ? 1 : 0; p >= 0; --p)
 #pragma unroll
                         for (int c = 0; c < KT / 16; ++c)
                             mma_f16_ta(tmem + COL_O + 128 * i, tmem + COL_S + 128 * i + 32 * (c >> 1) + 16 * p + 8 * (c & 1), vd + 128 * c, id_o,
-                                       (k >= 4 || c || p) ? 1u : 0u);
+                                       (k >= 4 || c || (TWO && p == 0)) ? 1u : 0u);
                     if (TWO || i) mma_commit(&sm.freed[n & 3]);
                     if (k >= items) mma_commit(&sm.ofull[i]);
                 }
@@ -232,14 +232,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int p = 0; p < (TWO ? 2 : 1); ++p)
+                    for (int p = TWO ? 1 : 0; p >= 0; --p)   // the small parts first: sums are truncated at every step
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
                             const uint64_t qd = sw128_desc(smem_u32(sm.q[TWO ? p : i][b]));
                             const uint64_t kd = sw128_desc(smem_u32(sm.kv[n & 3][b]));
 #pragma unroll
                             for (int c = 0; c < 4; ++c)
-                                mma_bf16(tmem + COL_S + 128 * i, qd + 2 * c, kd + 2 * c, id_s, (p || b || c) ? 1u : 0u);
+                                mma_bf16(tmem + COL_S + 128 * i, qd + 2 * c, kd + 2 * c, id_s, ((TWO && p == 0) || b || c) ? 1u : 0u);
                         }
                     mma_commit(&sm.sfull[i]);
                     if (TWO || i) mma_commit(&sm.freed[n & 3]);
