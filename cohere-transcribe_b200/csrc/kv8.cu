@@ -237,6 +237,24 @@ __global__ void __launch_bounds__(PT) count_kernel(const AllocArgs a) {
     if (threadIdx.x == 0) a.prefix[a.n] = before;
 }
 
+// Page p, the o-th free one, goes to the sequence with prefix[i] <= o < prefix[i + 1].
+__device__ __forceinline__ void take_page(const AllocArgs &a, int p, int o, int free_all) {
+    int lo = 0, hi = a.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.prefix[mid] <= o) lo = mid; else hi = mid;
+    }
+    if (a.prefix[lo + 1] > free_all) return;   // not all of its pages are there: none is taken
+    a.table[(size_t)lo * a.stride + a.first[lo] + (o - a.prefix[lo])] = p;
+    a.p.refs[p] = 1;
+}
+// The length of a sequence whose pages were there.
+__device__ __forceinline__ void grow(const AllocArgs &a, int i, int free_all) {
+    if (a.first[i] < 0) return;
+    if (a.prefix[i + 1] > a.prefix[i] && a.prefix[i + 1] > free_all) { set_status(CT_STATUS_NO_PAGE); return; }
+    a.len[i] = max(a.len[i], 0) + a.add[i];
+}
+
 // Hands the free pages out: the k-th lowest free page is the k-th asked for.
 template <bool FORK>
 __global__ void __launch_bounds__(PT) assign_kernel(const AllocArgs a) {
@@ -252,23 +270,56 @@ __global__ void __launch_bounds__(PT) assign_kernel(const AllocArgs a) {
         int total;
         const int o = at + cta_scan(f, total, sm);
         at += total;
-        if (!f || o >= asked) continue;
-        int lo = 0, hi = a.n;   // the sequence with prefix[i] <= o < prefix[i + 1]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.prefix[mid] <= o) lo = mid; else hi = mid;
-        }
-        if (a.prefix[lo + 1] > free_all) continue;   // not all of its pages are there: none is taken
-        a.table[(size_t)lo * a.stride + a.first[lo] + (o - a.prefix[lo])] = (int)p;
-        a.p.refs[p] = 1;
+        if (f && o < asked) take_page(a, (int)p, o, free_all);
     }
-    if (!FORK) {
-        for (int i = blockIdx.x * PT + threadIdx.x; i < a.n; i += gridDim.x * PT) {
-            if (a.first[i] < 0) continue;
-            if (a.prefix[i + 1] > a.prefix[i] && a.prefix[i + 1] > free_all) { set_status(CT_STATUS_NO_PAGE); continue; }
-            a.len[i] = max(a.len[i], 0) + a.add[i];
+    if (!FORK)
+        for (int i = blockIdx.x * PT + threadIdx.x; i < a.n; i += gridDim.x * PT) grow(a, i, free_all);
+}
+
+// Both steps in one CTA, for pools of at most SMALL pages: two launches less
+// (a beam step of 5 beams 16.4 -> 13.0 us) while one CTA's loads are short.
+constexpr int SMALL = 2 * PT;
+
+template <bool FORK>
+__global__ void __launch_bounds__(PT) alloc_kernel(const AllocArgs a) {
+    __shared__ int sm[32];
+    pdl_trigger();
+    int free_here[SMALL / PT], free_all = 0, asked = 0;
+#pragma unroll
+    for (int j = 0; j < SMALL / PT; ++j) {
+        const int p = j * PT + threadIdx.x;
+        free_here[j] = p < a.p.n_pages && a.p.refs[p] == 0;
+    }
+    for (int i0 = 0; i0 < a.n; i0 += PT) {
+        const int i = i0 + threadIdx.x;
+        int first = -1, total;
+        const int v = i < a.n ? pages_asked<FORK>(a, i, first) : 0;
+        const int at = cta_scan(v, total, sm);
+        if (i < a.n) {
+            a.first[i] = first;
+            a.prefix[i] = asked + at;
+            if (first < 0) set_status(CT_STATUS_BAD_ARG);
+        }
+        asked += total;
+    }
+    if (threadIdx.x == 0) a.prefix[a.n] = asked;
+    int rank[SMALL / PT];
+#pragma unroll
+    for (int j = 0; j < SMALL / PT; ++j) {
+        int total;
+        rank[j] = free_all;
+        if (j * PT < a.p.n_pages) {
+            rank[j] += cta_scan(free_here[j], total, sm);
+            free_all += total;
         }
     }
+    if (threadIdx.x == 0) a.seg[0] = free_all;
+    __syncthreads();   // the prefix is written
+#pragma unroll
+    for (int j = 0; j < SMALL / PT; ++j)
+        if (free_here[j] && rank[j] < asked) take_page(a, j * PT + threadIdx.x, rank[j], free_all);
+    if (!FORK)
+        for (int i = threadIdx.x; i < a.n; i += PT) grow(a, i, free_all);
 }
 
 // One page's slice of codes (16 bytes a thread) and, in slice 0, its scales.
@@ -397,6 +448,20 @@ __global__ void __launch_bounds__(PT) count_live_kernel(const CompactArgs a) {
 
 // With b(p) live pages below p: the free pages below L are numbered p - b(p),
 // the live ones from L on b(p) - b(L), and equal numbers pair up.
+__device__ __forceinline__ void plan_page(const CompactArgs &a, int p, int live, int b, int L) {
+    if (p >= a.p.n_pages) return;
+    if (p == L) a.head[1] = b;
+    int rank = -1;
+    if (p < L && !live) { a.dsts[p - b] = p; rank = -2; }
+    if (p >= L && live) { a.srcs[b] = p; rank = b; }
+    a.rank[p] = rank;
+}
+__device__ __forceinline__ void plan_head(const CompactArgs &a, int L) {
+    a.head[0] = L;
+    if (L == a.p.n_pages) a.head[1] = L;
+    if (a.n_live) *a.n_live = L;
+}
+
 __global__ void __launch_bounds__(PT) plan_kernel(const CompactArgs a) {
     __shared__ int sm[32];
     pdl_wait();
@@ -412,18 +477,31 @@ __global__ void __launch_bounds__(PT) plan_kernel(const CompactArgs a) {
         int total;
         const int b = at + cta_scan(live, total, sm);
         at += total;
-        if (!in) continue;
-        if (p == L) a.head[1] = b;
-        int rank = -1;
-        if (p < L && !live) { a.dsts[p - b] = p; rank = -2; }
-        if (p >= L && live) { a.srcs[b] = p; rank = b; }
-        a.rank[p] = rank;
+        if (in) plan_page(a, p, live, b, L);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        a.head[0] = L;
-        if (L == a.p.n_pages) a.head[1] = L;
-        if (a.n_live) *a.n_live = L;
+    if (blockIdx.x == 0 && threadIdx.x == 0) plan_head(a, L);
+}
+
+// Both steps in one CTA, for pools of at most SMALL pages.
+__global__ void __launch_bounds__(PT) plan_small_kernel(const CompactArgs a) {
+    __shared__ int sm[32];
+    pdl_trigger();
+    int live[SMALL / PT], below[SMALL / PT], L = 0;
+#pragma unroll
+    for (int j = 0; j < SMALL / PT; ++j) {
+        const int p = j * PT + threadIdx.x;
+        live[j] = p < a.p.n_pages && a.p.refs[p] > 0;
     }
+#pragma unroll
+    for (int j = 0; j < SMALL / PT; ++j) {
+        int total = 0;
+        below[j] = L;
+        if (j * PT < a.p.n_pages) below[j] += cta_scan(live[j], total, sm);
+        L += total;
+    }
+#pragma unroll
+    for (int j = 0; j < SMALL / PT; ++j) plan_page(a, j * PT + threadIdx.x, live[j], below[j], L);
+    if (threadIdx.x == 0) plan_head(a, L);
 }
 
 __global__ void __launch_bounds__(256) compact_kernel(const CompactArgs a, int slices) {
@@ -534,9 +612,6 @@ static int pool_map(CUtensorMap *map, const Pool &p) {
 }
 
 // ---- attention: which kernel, which tiles, which pieces
-#ifndef CT_KV8_FEW
-#define CT_KV8_FEW 64   // query rows of a sequence and kv head up to which few_kernel is taken
-#endif
 struct AttnPlan {
     int mt;          // few_kernel: tiles of 8 query rows per CTA; 0: many_kernel
     int tile;        // query rows of a CTA
@@ -552,7 +627,12 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
     if (window < 0 || window > (1 << 30) || sinks < 0 || sinks > (1 << 30) || (window && !causal)) return false;
     const long long rows = (long long)max_rows * (heads / c->kv_heads);   // query rows per kv head
     const int group = heads / c->kv_heads;
-    pl.mt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= CT_KV8_FEW ? 4 : 0;
+    // few_kernel up to 16 rows.  With 17 to 32 its CTAs (128 threads) only pay when
+    // sequences and heads alone fill the SMs: 20 bf16 rows of 4 heads a group, 16
+    // sequences of 20,000 keys 318 us against many_kernel's 382, 64 of 2000 keys 156
+    // against 187, but 4 of 8000 keys 86 against 54 and one of 2000 33 against 29.
+    // From 33 rows on it reads the cache twice: 571 us against 382.
+    pl.mt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 && (long long)s->n_seqs * c->kv_heads >= 128 ? 4 : 0;
     pl.tile = pl.mt ? 8 * pl.mt : type == CT_KV8_F32 ? 128 : 256;
     const long long tiles = (rows + pl.tile - 1) / pl.tile;
     long long list = pages_of(std::min<long long>(max_len, (long long)s->table_stride * ROWS));
@@ -646,6 +726,16 @@ static AllocArgs alloc_args(const ct_kv8_cache *c, const ct_kv8_seqs *s, void *w
     a.nseg = segments(c);
     return a;
 }
+template <bool FORK>
+static int launch_alloc(AllocArgs &a, cudaStream_t st) {
+    if (a.p.n_pages <= SMALL) {
+        a.nseg = 1;
+        return launch(alloc_kernel<FORK>, dim3(1), PT, 0, st, false, a);
+    }
+    int rc = launch(count_kernel<FORK>, dim3(a.nseg + 1), PT, 0, st, false, a);
+    if (rc == CT_OK) rc = launch(assign_kernel<FORK>, dim3(a.nseg), PT, 0, st, true, a);
+    return rc;
+}
 static bool good_ws(const void *ws) { return ws && (reinterpret_cast<uintptr_t>(ws) & 255) == 0; }
 
 }  // namespace kv8
@@ -722,9 +812,7 @@ extern "C" int ct_kv8_reserve(const ct_kv8_cache *c, const ct_kv8_seqs *s, const
     AllocArgs a = alloc_args(c, s, ws);
     a.add = add;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int rc = launch(count_kernel<false>, dim3(a.nseg + 1), PT, 0, st, false, a);
-    if (rc == CT_OK) rc = launch(assign_kernel<false>, dim3(a.nseg), PT, 0, st, true, a);
-    return rc;
+    return launch_alloc<false>(a, st);
 }
 
 extern "C" int ct_kv8_fork(const ct_kv8_cache *c, const ct_kv8_seqs *src, const int *parents, const ct_kv8_seqs *dst,
@@ -737,8 +825,7 @@ extern "C" int ct_kv8_fork(const ct_kv8_cache *c, const ct_kv8_seqs *src, const 
     a.src_table = src->table; a.src_len = src->len; a.parents = parents;
     a.src_stride = src->table_stride; a.src_n = src->n_seqs;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int rc = launch(count_kernel<true>, dim3(a.nseg + 1), PT, 0, st, false, a);
-    if (rc == CT_OK) rc = launch(assign_kernel<true>, dim3(a.nseg), PT, 0, st, true, a);
+    int rc = launch_alloc<true>(a, st);
     if (rc == CT_OK) rc = launch(fork_kernel, dim3(a.n, page_slices(a.p)), 256, 0, st, true, a);
     return rc;
 }
@@ -776,8 +863,13 @@ extern "C" int ct_kv8_compact(const ct_kv8_cache *c, const ct_kv8_seqs *s, int *
     a.seg = a.head + 2;
     a.nseg = segments(c);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int rc = launch(count_live_kernel, dim3(a.nseg), PT, 0, st, false, a);
-    if (rc == CT_OK) rc = launch(plan_kernel, dim3(a.nseg), PT, 0, st, true, a);
+    int rc;
+    if (c->n_pages <= SMALL) {
+        rc = launch(plan_small_kernel, dim3(1), PT, 0, st, false, a);
+    } else {
+        rc = launch(count_live_kernel, dim3(a.nseg), PT, 0, st, false, a);
+        if (rc == CT_OK) rc = launch(plan_kernel, dim3(a.nseg), PT, 0, st, true, a);
+    }
     if (rc == CT_OK) rc = launch(compact_kernel, dim3(148 * 4), 256, 0, st, true, a, page_slices(a.p));
     return rc;
 }
