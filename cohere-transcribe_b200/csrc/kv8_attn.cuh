@@ -20,6 +20,7 @@ struct AttnArgs {
     int causal, window, sinks;
     int chunk;              // pages of a piece
     int max_chunks;
+    int cluster;            // few_kernel: the pieces of a tile are one cluster and join through its shared memory
     float *part;            // [n_rows * heads][max_chunks][D], then [n_rows * heads][max_chunks][2]
 };
 
@@ -152,6 +153,7 @@ struct FewSmem {
     uint32_t q[MT][D / 16][32][QW];       // B fragments: high parts, low parts
     float qf[8 * MT];                     // per row: scale_log2 / its power of two
     float m[4][8 * MT], l[4][8 * MT];
+    float2 ml[8 * MT];                    // of the CTA, for the cluster's join
     uint64_t full[4][STAGES];
 };
 
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     const int t_lo = t_first + i0, t_hi = t_first + i0 + row_of(min(8 * MT, M - m0) - 1);
     const PageList list = page_list(a, len, t_lo, t_hi);
     const int pieces = list.n <= a.chunk ? 1 : (list.n + a.chunk - 1) / a.chunk;
-    if (piece >= pieces) return;
+    if (piece >= pieces && !a.cluster) return;   // a cluster's CTAs all stay for its barriers
 
     // this warp's pages: lane i holds the i-th one's number and block scales
     const int e1 = min(list.n, (piece + 1) * a.chunk);
@@ -527,6 +529,11 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
             const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][row][d]);
             acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
         }
+        if (a.cluster) {
+            *reinterpret_cast<float4 *>(&sm.o[0][row][d]) = acc;   // this thread alone reads and writes this place
+            if (d == 0) sm.ml[row] = make_float2(mx, lsum);
+            continue;
+        }
         const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
         const size_t r = (size_t)sp.first + i0 + qi;
         if (pieces == 1) {
@@ -539,6 +546,29 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
             if (d == 0) *reinterpret_cast<float2 *>(a.part + rows_all * a.max_chunks * D + b * 2) = make_float2(mx, lsum);
         }
     }
+    if (!a.cluster) return;
+    // The cluster's CTAs share out the tile's values; pieces in order.
+    cluster_sync();
+    for (int i = piece * 128 + threadIdx.x; i < 8 * MT * (D / 4); i += a.max_chunks * 128) {
+        const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (m0 + row >= M) break;
+        float mx = -INFINITY;
+        for (int c = 0; c < pieces; ++c) mx = fmaxf(mx, dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].x), c)));
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        float lsum = 0.0f;
+        float4 acc = make_float4(0, 0, 0, 0);
+        for (int c = 0; c < pieces; ++c) {
+            const float f = ex2(dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].x), c)) - ref);
+            lsum += dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].y), c)) * f;
+            const float4 x = dsmem_ld4(dsmem_addr(smem_u32(&sm.o[0][row][d]), c));
+            acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+        }
+        const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
+        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+        store4(static_cast<T *>(a.out) + ((size_t)sp.first + i0 + qi) * a.ldo + (size_t)h * D + d, acc.x * inv, acc.y * inv,
+               acc.z * inv, acc.w * inv);
+    }
+    cluster_sync();                       // nobody leaves while its results are being read
 }
 
 // Joins the pieces of each row: a warp per row, pieces in order.
@@ -567,7 +597,7 @@ __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, int tile_ro
         float l = 0.0f, acc[W];
 #pragma unroll
         for (int i = 0; i < W; ++i) acc[i] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (int c = 0; c < pieces; ++c) {
             const float2 x = ml[c];
             const float f = ex2(x.x - ref);
