@@ -21,7 +21,8 @@
  * default stream), never synchronise and allocate nothing, so all of them may be
  * captured into a CUDA graph; scratch space is the caller's (`ws`, 256-byte
  * aligned, no particular contents, not shared by calls that may overlap).  The
- * calls need no backend_init.  They return CT_OK, CT_EINVAL (a bad argument;
+ * calls need no backend_init.  Calls that change the same pages, tables, lengths
+ * or refs must be ordered by the caller (one stream, or events).  They return CT_OK, CT_EINVAL (a bad argument;
  * nothing was launched), CT_ENOMEM (ws too small; nothing was launched) or
  * CT_EDEVICE (a CUDA call failed, or an error was already pending).  What only
  * the device can see (a page number outside the pool, a length beyond the
@@ -53,7 +54,9 @@ extern "C" {
  *   scales [n_pages][n_layers][K, V][kv_heads], fp32
  * A value is code * scale of its block.  ct_kv8_append writes scales that are
  * powers of two; the attention takes any finite scale >= 0.  A scale of NaN
- * marks a block into which a NaN was written: all its values read as NaN.
+ * marks a block into which a NaN was written: all its values read as NaN.  The
+ * E4M3 codes 0x7F and 0xFF (NaN) are not used: rows below a sequence's length
+ * must not hold them, rows behind it may hold anything.
  *   refs   [n_pages]: how many sequences hold the page, 0 = free.  May be NULL
  * for ct_kv8_append and ct_kv8_attn, when the caller assigns pages itself.
  * head_dim is 64 or 128. */
@@ -65,7 +68,7 @@ typedef struct {
     int format;               /* CT_KV8_E4M3 or CT_KV8_INT8 */
 } ct_kv8_cache;
 
-/* Sequences: row s of `table` lists the pages of sequence s in order
+/* Sequences (at most 65535): row s of `table` lists the pages of sequence s in order
  * (token row t is row t % 16 of page table[s * table_stride + t / 16]); len[s]
  * is its number of token rows.  An entry of -1 is a page that was released. */
 typedef struct {
@@ -107,10 +110,12 @@ int ct_kv8_append(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const 
  * out that belong to no sequence are left as they were.
  * max_rows, max_len: upper bounds of the rows and of len[s] of any sequence
  * (when one is exceeded that sequence's rows of out are left as they were: status).
- * Products, sums and the softmax are fp32 (K and V codes exactly; fp32 queries
- * and probabilities as pairs of fp16, 22 bits; in calls of many bf16 rows the
- * probabilities as one fp16).  A result does not depend on the other sequences'
- * contents.  ws: at least ct_kv8_attn_ws_bytes of the same arguments. */
+ * Products, sums and the softmax are fp32; K and V codes enter them exactly,
+ * queries and probabilities as fp16 numbers scaled by powers of two: two each
+ * (22 bits) for fp32 rows, one (11 bits, which holds a bf16 query exactly) for
+ * bf16 rows.  A result depends on the sizes of the call, not on the other
+ * sequences' contents, and is the same each time.  out may be q itself.
+ * ws: at least ct_kv8_attn_ws_bytes of the same arguments. */
 int ct_kv8_attn(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const void *q, int ldq, void *out, int ldo,
                 int type, int n_rows, const int *row_start, int max_rows, int max_len, int heads, float scale,
                 int causal, int window, int sinks, void *ws, size_t ws_bytes, void *stream);
@@ -169,7 +174,8 @@ size_t ct_kv8_pages_ws_bytes(const ct_kv8_cache *c, int n_seqs);
 
 /* Waits for the current device, then reads and clears its status word
  * (0 = nothing reported, 4 = something was out of range and left out, 6 = no
- * free page was left); CT_EDEVICE when a CUDA call failed.  The word is the
+ * free page was left, 1 to 3 = a bounded wait inside a kernel gave up: its output
+ * is not to be used); CT_EDEVICE when a CUDA call failed.  The word is the
  * library's own, one per device: ct_device_status and ct_engine_status read the
  * same one. */
 int ct_kv8_status(void);

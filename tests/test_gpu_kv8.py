@@ -255,6 +255,43 @@ def test_attention_many_rows(kv8, fmt, typ, kvh, heads, dim, rows, past):
     check_attend(kv8, c, s, rc, table, lens, rows, heads, typ, window=1, sinks=0)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_many_sequences_of_some_rows(kv8, fmt, typ, dim):
+    """17 to 32 rows per kv head with enough sequences to fill the GPU: a kernel form of its own."""
+    rng = np.random.default_rng(dim)
+    rows = [6 if i == 3 else int(rng.integers(0, 7)) for i in range(70)]
+    lens = [r + int(rng.integers(0, 120)) for r in rows]
+    lens[5] = 1500 + rows[5]
+    c, s, rc, table = make(kv8, fmt, lens, 2, dim, seed=dim)
+    check_attend(kv8, c, s, rc, table, lens, rows, 10, typ)
+    check_attend(kv8, c, s, rc, table, lens, rows, 10, typ, window=33, sinks=2)
+
+
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads", [17, 40, 128, 300])
+def test_attention_large_groups(kv8, typ, heads):
+    """One row per sequence, many heads on one kv head: odd groups, tiles that end inside a query row."""
+    lens = [70, 1, 300]
+    c, s, rc, table = make(kv8, "int8", lens, 1, 64, seed=heads)
+    check_attend(kv8, c, s, rc, table, lens, [1, 1, 1], heads, typ)
+    check_attend(kv8, c, s, rc, table, lens, [1, 1, 1], heads, typ, window=20, sinks=1)
+
+
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows", [1, 3, 200])
+def test_attention_in_place(kv8, torch, typ, rows):
+    """out may be q: the same bits as into another tensor, with and without pieces to join."""
+    for n in (40, 400, 3000):
+        c, s, rc, table = make(kv8, "e4m3", [n + rows, rows], 2, 128)
+        q = torch.randn(2 * rows, 4, 128, device="cuda").to(getattr(torch, typ))
+        st = dev([0, rows, 2 * rows])
+        want = c.attend(1, s, q, row_start=st, max_rows=rows)
+        c.attend(1, s, q, out=q, row_start=st, max_rows=rows)
+        assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("typ", ["float32", "bfloat16"])
 @pytest.mark.parametrize("rows", [1, 6, 300])
 def test_attention_window_over_a_long_cache(kv8, typ, rows):
