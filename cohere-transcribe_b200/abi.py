@@ -1,4 +1,4 @@
-"""ctypes prototypes of libct_b200.so (the C ABI of include/ct_backend.h).
+"""ctypes prototypes of libct_b200.so (the C ABI of include/*.h).
 
 `load()` fails loudly when the library is missing: there is no CPU path.
 """

@@ -136,6 +136,11 @@ __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d)
 // Each warp keeps a few pages in flight through a ring of its own, one TMA
 // copy per K and V block; TMA's swizzle spreads both access patterns over all
 // banks.
+//
+// Bound by HBM where there is much to read (16 rows of 32 heads over 8k to 65k keys:
+// 1.19 GB in 205 us, 5.8 TB/s), otherwise by latency: a pair of pages takes a warp
+// 3 to 4 thousand cycles among 16 warps, and start and join about 6 thousand (64
+// rows over up to 1024 keys: 31 us for 62 MB; one row over 376 keys: 9.3 us).
 // Pages in flight per warp, and CTAs per SM.  8 rows of 128 dims: 3 pages and 4
 // CTAs are 2 to 3% faster than 4 pages and 3 CTAs (attention of 16 rows over 8k to
 // 65k keys 207.5 against 213.2 us).
@@ -316,6 +321,7 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) c[mt][n][0] = c[mt][n][1] = c[mt][n][2] = c[mt][n][3] = 0.0f;
+            float small[MT][4] = {};      // the low parts' sums: the tensor core truncates, so they stay apart
             const uint8_t *kp = sm.kv[warp][(it + n) % STAGES][0];
             uint4 k[2][KC];
 #pragma unroll
@@ -340,12 +346,18 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
                     if (TWO) {
                         const uint4 f = *reinterpret_cast<const uint4 *>(q);
                         mma_f16(c[mt][n], ka, f.x, f.y);
-                        mma_f16(c[mt][n], ka, f.z, f.w);
+                        mma_f16(small[mt], ka, f.z, f.w);
                     } else {
                         const uint2 f = *reinterpret_cast<const uint2 *>(q);
                         mma_f16(c[mt][n], ka, f.x, f.y);
                     }
                 }
+            }
+            if (TWO) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[mt][n][e] += small[mt][e];
             }
         }
         // every row of the tile sees all of both pages
@@ -482,8 +494,16 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
                     const uint32_t va[4] = {x[0][2 * d], x[0][2 * d + 1], x[1][2 * d], x[1][2 * d + 1]};
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        mma_f16(o[mt][w * 2 + d], va, ph[mt][n][0], ph[mt][n][1]);
-                        if (TWO) mma_f16(o[mt][w * 2 + d], va, pl[mt][n][0], pl[mt][n][1]);
+                        float (&acc)[4] = o[mt][w * 2 + d];
+                        if (TWO) {        // a page's sum alone on the tensor core, small parts first; rounded into the rest
+                            float x4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(x4, va, pl[mt][n][0], pl[mt][n][1]);
+                            mma_f16(x4, va, ph[mt][n][0], ph[mt][n][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[e] += x4[e];
+                        } else {
+                            mma_f16(acc, va, ph[mt][n][0], ph[mt][n][1]);
+                        }
                     }
                 }
             }
@@ -571,7 +591,9 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     cluster_sync();                       // nobody leaves while its results are being read
 }
 
-// Joins the pieces of each row: a warp per row, pieces in order.
+// Joins the pieces of each row: a warp per row, pieces in order, eight loads in
+// flight (3 us for 512 rows of two pieces; launch latency is hidden behind the
+// kernel before it).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, int tile_rows) {
     pdl_wait();
