@@ -43,7 +43,9 @@ namespace kv8 {
 
 // Warps 0..3: MMA issue (warp 0); 4..7: codes -> fp16; 8..15: the streams.  A
 // softmax thread keeps its row's 128 scores in registers, so the warpgroups
-// split the launch's 4 x 128 registers per lane as 40 + 104 + 184 + 184.
+// split the launch's 4 x 128 registers per lane as 40 + 104 + 184 + 184 (the MMA
+// thread is on the critical path: with 24 registers windowed fp32 prompts take 352
+// us instead of 283, and its loop over the two parts stays rolled, 275).
 constexpr int MANY_THREADS = 512;
 constexpr int KT = 128;             // keys of a tile
 constexpr int KB = KT / ROWS;       // blocks of a tile
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = sw128_mn_desc(smem_u32(sm.kv[n & 3][0]));
-#pragma unroll
+#pragma unroll 1
                     for (int p = TWO ? 1 : 0; p >= 0; --p)
 #pragma unroll
                         for (int c = 0; c < KT / 16; ++c)
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                     ok = many_wait(&sm.full[n & 3], (n >> 2) & 1, CT_STATUS_TIMEOUT_TMA);
                     if (!ok) break;
                     tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                     for (int p = TWO ? 1 : 0; p >= 0; --p)   // the small parts first: sums are truncated at every step
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
