@@ -453,7 +453,11 @@ def main():
     if args.impl == "reference":
         if rank != 0:
             return
-        ref = ReferenceCPU(case, enc, audio, ncores, args.cpu_tokens)
+        try:
+            ref = ReferenceCPU(case, enc, audio, ncores, args.cpu_tokens)
+        except RuntimeError as e:
+            print(json.dumps({"impl": "reference", "unavailable": str(e)}), flush=True)
+            return
         for _ in range(args.warmup):
             ref.decode(warm=True)
         toks, secs, aud, tsecs = 0, 0.0, 0.0, 0.0
