@@ -674,10 +674,12 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
         // whole key tiles; one piece once the tiles alone give every SM a CTA
         long long pieces = std::min(std::max(1ll, 148 / ctas), std::max(1ll, list / (4 * KB)));
         // The tensor core truncates each of its fp32 sums, so an error grows with the
-        // keys summed into one accumulator.  fp32 results take at most 2048 keys a
-        // piece (a sixteenth of them past 32,768) and join the pieces with rounded
-        // sums: against 64 bits 1.0e-6 instead of 2.1e-6 at 4000 keys.
-        if (type == CT_KV8_F32) pieces = std::max(pieces, std::min(16ll, (list + 127) / 128));
+        // keys summed into one accumulator.  fp32 results take at most 1024 keys a
+        // piece (1280 where that saves cutting, a sixteenth of them past 16,384) and
+        // join the pieces with rounded sums: 4 of 1842 drawn calls are further from 64
+        // bits than 1e-6 and 1.5 times torch's fp32 products, with pieces of 2048 keys
+        // 24 of 1412 (4 prompts of 1000 to 4097 rows take 2605 us instead of 2066).
+        if (type == CT_KV8_F32 && list > 80) pieces = std::max(pieces, std::min(16ll, (list + 63) / 64));
         chunk = ((list + pieces - 1) / pieces + KB - 1) / KB * KB;
     }
     pl.chunk = (int)chunk;
