@@ -19,7 +19,7 @@ namespace kv8 {
 // The loads hang together as length -> rows and page -> scale, so the rows are
 // under way before the page is known.  Bound by the latency of that chain: a
 // decode step of 256 sequences takes 8.3 us (1.6 MB), prompts of 56k bf16 rows
-// 82 us (363 MB, 4.4 TB/s; with 6 instead of 8 CTAs per SM 86, with 10 92 us).
+// 81 us (363 MB, 4.5 TB/s; with 6 instead of 8 CTAs per SM 86, with 10 92 us).
 struct AppendArgs {
     Pool p;
     const int *table, *len, *row_start;
@@ -687,7 +687,7 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
     pl.max_chunks = (int)((list + chunk - 1) / chunk);
     if (tiles * pl.max_chunks > INT_MAX) return false;
     // Up to 8 pieces of a tile are one cluster when all CTAs fit the SMs at once: no
-    // second kernel (one row over 376 keys 10.9 -> 9.3 us).
+    // second kernel (one row over 376 keys: 1.5 us less).
     pl.cluster = pl.mt && pl.max_chunks > 1 && pl.max_chunks <= 8 && ctas * pl.max_chunks <= at_once;
     pl.ws = pl.max_chunks > 1 && !pl.cluster ? (size_t)n_rows * heads * pl.max_chunks * (c->head_dim + 2) * sizeof(float) : 0;
     return true;

@@ -27,7 +27,7 @@
 // scores hold their high parts in the first 16 and their low parts in the rest.
 //
 // Measured: 4 prompts of 1000 to 4097 bf16 rows, 32 heads on 8, 679 GFLOP in 897 us
-// (757 TFLOP/s); windowed fp32 prompts, 62 GFLOP (every product as two MMAs), 283
+// (757 TFLOP/s); windowed fp32 prompts, 62 GFLOP (every product as two MMAs), 276
 // us.  No unit is the bound (tensor pipe 38%, exponentials 39%, issue slots 42%): a
 // stream's chain is, about 3.1 thousand cycles of softmax and 2 thousand until its
 // next scores are there, per tile of 128 keys.  128 keys a tile keep the chain's

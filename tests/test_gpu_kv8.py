@@ -422,6 +422,26 @@ def test_attention_does_not_depend_on_the_other_sequences(kv8, torch, typ, rows)
     assert torch.equal(a[rows:2 * rows], b[rows:2 * rows])
 
 
+@pytest.mark.parametrize("rows", [1, 4, 100])
+def test_attention_on_two_streams(kv8, torch, rows):
+    """Two calls over the same cache at once, each with a workspace of its own: the bits of one call alone."""
+    c, s, rc, table = make(kv8, "e4m3", [3000 + rows, 700 + rows, rows], 2, 128)
+    st = dev(starts_of([rows] * 3))
+    qs = [torch.randn(3 * rows, 4, 128, device="cuda") for _ in range(2)]
+    want = [c.attend(1, s, q, row_start=st, max_rows=rows) for q in qs]
+    ws = [c.attend_workspace(s, q, max_rows=rows) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for q, w, stream in zip(qs, ws, streams):
+            with torch.cuda.stream(stream):
+                got.append(c.attend(1, s, q, row_start=st, max_rows=rows, ws=w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert c.status() == 0
+
+
 def test_offsets_beyond_32_bits(kv8, torch):
     """Pages whose byte offsets pass 2^32: written, read, copied and moved there."""
     pages, layers, kvh, dim = 20000, 4, 16, 128      # 256 KB each: 5.2 GB
