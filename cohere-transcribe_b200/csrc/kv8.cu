@@ -665,10 +665,13 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
     const long long at_once = 148 * few_ctas(pl.mt);
     long long chunk;
     if (pl.mt) {
-        // As many pieces as the SMs hold CTAs at once, each warp with two pages at
-        // least (4 rows of one sequence of 8000 keys: 22.6 us against 36.2 with twice
-        // the pieces); a rest of up to a quarter of a piece is not cut off.
-        chunk = std::min<long long>(FEW_CHUNK, (std::max(1ll, ctas * list / at_once) + 7) / 8 * 8);
+        // Pieces of equal length, the most with which all CTAs run at once, three on an
+        // SM (two of 32-row tiles), each warp with two pages at least.  4 rows of one
+        // sequence of 8000 keys: 16.6 us; 22.7 with four CTAs on an SM, 36.2 with twice
+        // as many as fit.  32 windows of 2048 keys, 16 rows each: 23 us, 33 with 640
+        // CTAs, of which 444 fit.  A rest of up to a quarter is not cut off.
+        const long long pieces = std::max({1ll, 148 * std::min(3, few_ctas(pl.mt)) / ctas, (list + FEW_CHUNK - 1) / FEW_CHUNK});
+        chunk = ((list + pieces - 1) / pieces + 7) / 8 * 8;
         if (list <= chunk + chunk / 4) chunk = std::min<long long>(FEW_CHUNK, (list + 3) / 4 * 4);
     } else {
         // whole key tiles; one piece once the tiles alone give every SM a CTA
