@@ -12,9 +12,11 @@
 //   are joined at the end like two pieces of a split.
 // While one stream's rows are in their softmax the tensor core works for the
 // other: step k issues P.V of item k - 2 and Q.K of item k, where items
-// alternate between the streams.  The MMAs of one thread complete in order, so
-// a finished Q.K of a stream means that its earlier P.V is finished as well,
-// and O may be rescaled and S overwritten by P without further waits.
+// alternate between the streams.  Two MMAs of one thread are ordered only when they
+// share accumulator and shape (the PTX ISA's list of pipelined tcgen05 pairs), so
+// Q.K of item k, which overwrites the P that P.V of item k - 2 reads, waits for that
+// P.V (pdone).  A commit covers all earlier MMAs of its thread: once scores are
+// there (sfull), the stream's O may be rescaled and S overwritten by P.
 //
 // Operands: Q as fp16, each row scaled by a power of two.  Codes are exact in
 // fp16: a warpgroup loads them from global memory a tile ahead, converts, and
@@ -59,7 +61,7 @@ struct ManySmem {
     int base[4][KB];                     // first token row of each block; ABSENT = not there
     float qf[256];                       // per row: scale_log2 / power of two of its query
     float join[3][128];
-    uint64_t full[4], freed[4], sfull[2], pfull[2], ofull[2], qfull;
+    uint64_t full[4], freed[4], sfull[2], pfull[2], pdone[2], ofull[2], qfull;
     uint32_t tmem;
 };
 
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) { mbar_init(&sm.full[i], 128); mbar_init(&sm.freed[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sm.sfull[i], 1); mbar_init(&sm.pfull[i], 128); mbar_init(&sm.ofull[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sm.sfull[i], 1); mbar_init(&sm.pfull[i], 128); mbar_init(&sm.pdone[i], 1); mbar_init(&sm.ofull[i], 1); }
         mbar_init(&sm.qfull, 256);
         fence_mbar_init();
     }
@@ -234,11 +236,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                             mma_f16_ta(tmem + COL_O + 128 * i, tmem + COL_S + 128 * i + 32 * (c >> 1) + 16 * p + 8 * (c & 1), vd + 128 * c, id_o,
                                        (k >= 4 || c || (TWO && p == 0)) ? 1u : 0u);
                     if (TWO || i) mma_commit(&sm.freed[n & 3]);
-                    if (k >= items) mma_commit(&sm.ofull[i]);
+                    mma_commit(k < items ? &sm.pdone[i] : &sm.ofull[i]);
                 }
                 if (k < items) {
                     const int j = TWO ? k : k >> 1, n = 2 * j;
-                    ok = many_wait(&sm.full[n & 3], (n >> 2) & 1, CT_STATUS_TIMEOUT_TMA);
+                    ok = many_wait(&sm.full[n & 3], (n >> 2) & 1, CT_STATUS_TIMEOUT_TMA) &&
+                         (k < 2 || many_wait(&sm.pdone[i], ((k - 2) >> 1) & 1, CT_STATUS_TIMEOUT_MMA));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1

@@ -255,6 +255,17 @@ def test_attention_many_rows(kv8, fmt, typ, kvh, heads, dim, rows, past):
     check_attend(kv8, c, s, rc, table, lens, rows, heads, typ, window=1, sinks=0)
 
 
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_many_rows_over_many_key_tiles(kv8, typ, dim):
+    """Pieces of many key tiles: every tile's scores take the place of the tile's probabilities before it."""
+    rows, past = [300, 40, 130, 7], [3700, 2461, 0, 900]
+    lens = [a + b for a, b in zip(rows, past)]
+    c, s, rc, table = make(kv8, "e4m3", lens, 4, dim, seed=dim)
+    check_attend(kv8, c, s, rc, table, lens, rows, 8, typ)
+    check_attend(kv8, c, s, rc, table, lens, rows, 8, typ, window=1500, sinks=40)
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("typ", ["float32", "bfloat16"])
 @pytest.mark.parametrize("dim", [64, 128])
