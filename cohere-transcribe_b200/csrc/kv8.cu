@@ -550,16 +550,19 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const Pool p, const int
 }
 
 // ---- host side ------------------------------------------------------------------
+static bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 static bool good_cache(const ct_kv8_cache *c) {
-    return c && c->codes && c->scales && c->n_pages > 0 && c->n_layers > 0 && c->n_layers <= 4096 && c->kv_heads > 0 &&
-           c->kv_heads <= 4096 && (c->head_dim == 64 || c->head_dim == 128) &&
-           (c->format == CT_KV8_E4M3 || c->format == CT_KV8_INT8) &&
-           (long long)c->n_pages * c->n_layers * c->kv_heads < (1ll << 30) &&   // blocks are numbered in 31 bits (reinterpret_cast<uintptr_t>(c->codes) & 15) == 0 &&
-           (reinterpret_cast<uintptr_t>(c->scales) & 3) == 0;
+    if (!c || !c->codes || !c->scales || c->n_pages <= 0 || c->n_layers <= 0 || c->n_layers > 4096 || c->kv_heads <= 0 ||
+        c->kv_heads > 4096 || (c->head_dim != 64 && c->head_dim != 128) ||
+        (c->format != CT_KV8_E4M3 && c->format != CT_KV8_INT8))
+        return false;
+    // blocks are numbered in 31 bits
+    if ((long long)c->n_pages * c->n_layers * c->kv_heads >= (1ll << 30)) return false;
+    return aligned(c->codes, 16) && aligned(c->scales, 4) && aligned(c->refs, 4);
 }
 static bool good_seqs(const ct_kv8_seqs *s) {
     return s && s->table && s->len && s->n_seqs > 0 && s->n_seqs <= 65535 && s->table_stride > 0 &&
-           s->table_stride <= (1 << 26);
+           s->table_stride <= (1 << 26) && aligned(s->table, 4) && aligned(s->len, 4);
 }
 static Pool pool_of(const ct_kv8_cache *c) {
     return Pool{c->codes, c->scales, c->refs, c->n_pages, c->n_layers, c->kv_heads, c->head_dim};
@@ -567,7 +570,7 @@ static Pool pool_of(const ct_kv8_cache *c) {
 // rows of `width` values with stride ld: vectors of 16 bytes
 static bool good_rows(const void *p, int ld, long long width, int type) {
     const int size = type == CT_KV8_F32 ? 4 : 2;
-    return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld >= width && ((long long)ld * size) % 16 == 0;
+    return p && aligned(p, 16) && ld >= width && ((long long)ld * size) % 16 == 0;
 }
 
 // A kernel launch that reports a pending or a new error as a code; `pdl`: may
@@ -770,7 +773,7 @@ static int launch_alloc(AllocArgs &a, cudaStream_t st) {
     if (rc == CT_OK) rc = launch(assign_kernel<FORK>, dim3(a.nseg), PT, 0, st, true, a);
     return rc;
 }
-static bool good_ws(const void *ws) { return ws && (reinterpret_cast<uintptr_t>(ws) & 255) == 0; }
+static bool good_ws(const void *ws) { return ws && aligned(ws, 256); }
 
 }  // namespace kv8
 }  // namespace ct

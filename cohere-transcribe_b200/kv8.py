@@ -71,8 +71,9 @@ class Cache:
 
     def __init__(self, codes, scales, refs=None, fmt="e4m3"):
         _need(codes.dtype == torch.uint8 and codes.dim() == 6 and codes.is_contiguous() and codes.is_cuda
-              and codes.shape[2] == 2 and codes.shape[4] == ROWS and codes.shape[5] in (64, 128),
-              "codes: a contiguous uint8 tensor [pages, layers, 2, kv_heads, 16, 64 or 128] on a GPU")
+              and codes.shape[2] == 2 and codes.shape[4] == ROWS and codes.shape[5] in (64, 128)
+              and codes.data_ptr() % 16 == 0,
+              "codes: a contiguous uint8 tensor [pages, layers, 2, kv_heads, 16, 64 or 128] on a GPU, 16-byte aligned")
         _need(scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == codes.shape[:4]
               and scales.device == codes.device, "scales: a contiguous float32 tensor [pages, layers, 2, kv_heads]")
         _need(fmt in FORMATS, "fmt: 'e4m3' or 'int8'")

@@ -59,7 +59,8 @@ extern "C" {
  * must not hold them, rows behind it may hold anything.
  *   refs   [n_pages]: how many sequences hold the page, 0 = free.  May be NULL
  * for ct_kv8_append and ct_kv8_attn, when the caller assigns pages itself.
- * head_dim is 64 or 128. */
+ * head_dim is 64 or 128; n_layers and kv_heads are 4096 at most, and
+ * n_pages * n_layers * kv_heads is below 2^30. */
 typedef struct {
     uint8_t *codes;
     float *scales;

@@ -644,6 +644,15 @@ def test_python_checks_arguments(kv8, torch):
         assert e.value.code == -1
 
 
+def test_python_refuses_a_misaligned_pool(kv8, torch):
+    arena = torch.zeros(2 * 2 * ROWS * 64 + 16, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(2, 1, 2, 1, device="cuda")
+    for at in (1, 4, 8):
+        with pytest.raises(ValueError):
+            kv8.Cache(arena[at:at + 2 * 2 * ROWS * 64].view(2, 1, 2, 1, ROWS, 64), scales)
+    kv8.Cache(arena[16:].view(2, 1, 2, 1, ROWS, 64), scales)
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 def test_beam_search_run(kv8, torch, fmt):
     """Prompts, then steps of reserve / append / attend / fork / free / trim / compact as a beam search makes them,

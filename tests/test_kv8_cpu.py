@@ -103,6 +103,24 @@ def test_bad_sequences_are_refused(lib, args, bad):
     assert lib.ct_kv8_compact(r, p, args.a, args.a, None, args.a, 4096, None) == CT_EINVAL
 
 
+@pytest.mark.parametrize("field,offset", [("codes", 1), ("codes", 8), ("scales", 1), ("scales", 2)])
+def test_misaligned_pools_are_refused(lib, args, field, offset):
+    """codes by 16 bytes, scales by 4: the kernels read them that wide."""
+    c, s = args.cache(**{field: args.a + offset}), args.seqs()
+    assert _append(lib, args, cache=c) == CT_EINVAL
+    assert _attn(lib, args, cache=c) == CT_EINVAL
+    r, p = ctypes.byref(c), ctypes.byref(s)
+    t = ctypes.byref(args.seqs(table=args.a + 256, len=args.a + 512))
+    assert lib.ct_kv8_pages_ws_bytes(r, 3) == 0
+    assert lib.ct_kv8_attn_ws_bytes(r, p, 0, 9, 4, 64, 4, 1, 0, 0) == 0
+    assert lib.ct_kv8_reserve(r, p, args.a, args.a, 4096, None) == CT_EINVAL
+    assert lib.ct_kv8_fork(r, p, args.a, t, args.a, 4096, None) == CT_EINVAL
+    assert lib.ct_kv8_free(r, p, None, 0, None) == CT_EINVAL
+    assert lib.ct_kv8_trim(r, p, 16, 0, None) == CT_EINVAL
+    assert lib.ct_kv8_compact(r, p, args.a, args.a, None, args.a, 4096, None) == CT_EINVAL
+    assert lib.ct_kv8_copy_pages(r, args.a, args.a, 1, None) == CT_EINVAL
+
+
 @pytest.mark.parametrize("bad", [
     dict(layer=-1), dict(layer=2), dict(k=None), dict(v=None), dict(ldk=127), dict(ldv=126), dict(ldk=130),
     dict(type=2), dict(n_rows=0), dict(max_rows=0), dict(max_rows=(1 << 20) + 1), dict(rs=None),
