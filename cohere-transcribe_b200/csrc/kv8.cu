@@ -200,7 +200,7 @@ __device__ __forceinline__ int pages_asked(const AllocArgs &a, int i, int &first
         if (q >= a.src_n) return 0;
         const int len = a.src_len[q];
         if (len <= 0) { first = 0; return 0; }
-        if (pages_of(len) > a.stride || pages_of(len) > a.src_stride) return 0;
+        if (len > min(a.stride, a.src_stride) * ROWS) return 0;   // before pages_of, which adds to it
         if (len % ROWS == 0) { first = 0; return 0; }
         if (!a.p.has(a.src_table[(size_t)q * a.src_stride + len / ROWS])) return 0;
         first = len / ROWS;

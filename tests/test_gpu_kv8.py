@@ -543,6 +543,22 @@ def test_fork(kv8, torch, pages, seqs, width, kids):
     assert s.table.tolist() == table and s.lens.tolist() == lens
 
 
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16, 2 ** 30, 5 * ROWS + 1, 4 * ROWS + 1])
+def test_fork_leaves_out_lengths_beyond_the_tables(kv8, torch, length):
+    """A parent's length that its table, or the child's, does not hold: the child ends empty, the others do not."""
+    c = kv8.Cache.empty(40, 1, 1, 64, "int8")
+    s, d = kv8.Seqs.empty(2, 5), kv8.Seqs(dev([[-7] * 4] * 2), dev([0, 0]))
+    c.reserve(s, dev([20, 20]))
+    s.lens[0] = length
+    refs = c.refs.tolist()
+    c.fork(s, dev([0, 1]), d)
+    assert c.status() == BAD_ARG and d.lens.tolist() == [0, 20] and d.table[0].tolist() == [-7] * 4
+    full, free = s.table[1, 0].item(), refs.index(0)
+    assert d.table[1].tolist() == [full, free, -7, -7]
+    refs[full], refs[free] = 2, 1
+    assert c.refs.tolist() == refs
+
+
 def test_free_and_its_indices(kv8):
     c, s, table, lens, refs = pool(kv8, 400, 50, 9, 5)
     which = [3, 7, 3, 49, 0, 7]
