@@ -82,9 +82,49 @@ __device__ __forceinline__ float row_pow2(float amax) {
 }
 // 1 / x of a power of two in [2^-126, 2^126], without a division.
 __device__ __forceinline__ float inv_pow2(float x) { return __uint_as_float(0x7F000000u - __float_as_uint(x)); }
-// The power of two that O is held in for block scales up to vmax.
-__device__ __forceinline__ float o_unit(float vmax) {
-    return fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7F800000u), 1.1754944e-38f), 8.5070592e37f);
+
+// ---- softmax state of a row, both kernels
+// Scores x are in log2.  m is the reference of the exponentials, an integer, so that
+// moving it scales by exact powers of two; it moves when a score passes it by THR.
+// A key's probability p = 2^(x - m + OFF) goes into the sum l, and
+// p vs / 2^e (vs: the block scale of its V) as fp16 into P.V.  The exponent e of the
+// unit that O is held in follows the largest product of probability and scale, not the
+// scales alone: a block with a large scale and next to no probability must not push
+// the others' products below what fp16 holds.  With
+//   need = max over blocks (largest score - m + log2 vs),
+// e is raised to need when that passes it by SLACK and comes down with every move of m.
+// So the largest product lies in [2^(OFF - 1), 2^(OFF + SLACK + 1)] <= 2^15 when it is
+// seen, and an fp16's absolute step is 2^-32 of it.  Scores more than 120 below m count as
+// 120 in need: then vs / 2^e stays finite (such a p is 2^-111 at most).
+// e stays within [-126, 126]: at 126, with vs < 2^128, need <= 127 + THR = 126 + SLACK.
+constexpr float THR = 4.0f, OFF = 9.0f, SLACK = 5.0f, FAR = -120.0f;
+constexpr float E_MIN = -126.0f, E_MAX = 126.0f;
+// 2^x of an integer in [-127, 127]; 0 for -127: the sum's low bits hold 127 + x
+__device__ __forceinline__ float pow2i(float x) { return __uint_as_float(__float_as_uint(x + 12583039.0f) << 23); }
+// floor(log2 v) of v >= 0 (-127 for 0 and subnormals)
+__device__ __forceinline__ float log2_floor(float v) {
+    return __uint_as_float(0x4B400000u | (__float_as_uint(v) >> 23 & 0xFFu)) - 12583039.0f;
+}
+// Whether a row with largest new score mx, over blocks with V scales up to 2^(lv + 1), may
+// have to move m or raise e (an upper bound of need decides).
+__device__ __forceinline__ bool unsettled(float mx, float lv, float m, float e) {
+    const float d = mx - m;
+    return d > THR || fmaxf(d, FAR) + lv > e + SLACK;
+}
+// The new m, and what the sums so far are multiplied by for it.
+__device__ __forceinline__ float move_m(float mx, float &m) {
+    const bool move = mx > m + THR;                // always once a first key is seen
+    const float mn = move ? ceilf(mx) : m, d = move ? fmaxf(m - mn, -300.0f) : 0.0f;
+    m = mn;
+    return d;                                      // a power of two's exponent
+}
+// The new e after m moved by d, and the exponent of what O is multiplied by (<= 0).
+__device__ __forceinline__ float move_e(float need, float d, float &e) {
+    const float down = fmaxf(e + d, E_MIN);
+    const float en = need > down + SLACK ? fminf(ceilf(need), E_MAX) : down;
+    const float f = fmaxf(d + e - en, -127.0f);
+    e = en;
+    return f;
 }
 
 template <typename T>
@@ -128,10 +168,8 @@ __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d)
 // 4 consecutive bytes per MMA, and V's 16 rows are neighbouring dims of the 16
 // (8) that lane group g loaded.  P^T comes from S^T by 8 x 8 transposes.
 //
-// The reference of a row's exponentials moves only when some score passes it by
-// 2^THR, so most pages need one vote and no shuffles; V's block scale goes into
-// the probabilities, relative to a power of two E per row that O is held in and
-// that moves the same way.  P = 2^(x - reference + OFF) vs / E <= 2^15.
+// The reference of a row's exponentials and the unit of its O move seldom, so most
+// pages need one vote and no shuffles.
 //
 // Each warp keeps a few pages in flight through a ring of its own, one TMA
 // copy per K and V block; TMA's swizzle spreads both access patterns over all
@@ -176,7 +214,6 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     constexpr int KS = D / 16;            // MMA steps of Q.K
     constexpr int NJ = D / 16;            // MMA row tiles of P.V
     constexpr int VB = D / 8;             // V bytes per key and lane
-    constexpr float THR = 4.0f, OFF = 7.0f;
     extern __shared__ __align__(1024) uint8_t few_raw[];
     FewSmem<T, D, MT> &sm = *reinterpret_cast<FewSmem<T, D, MT> *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -276,7 +313,7 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     __syncthreads();
 
     float o[MT][NJ][4];                   // dims 2 j, 2 j + 1 of the lane group's, rows 2 t, 2 t + 1: (d, r), (d, r'), (d', r), (d', r')
-    float mref[MT][2], l[MT][2], E[MT][2], qf[MT][2];
+    float mref[MT][2], l[MT][2], eo[MT][2], qf[MT][2];
     int tq[MT][2];                        // token row of this lane's query rows
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -285,7 +322,7 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
             const int m = m0 + mt * 8 + 2 * t + e;
             mref[mt][e] = -INFINITY;
             l[mt][e] = 0.0f;
-            E[mt][e] = 1.1754944e-38f;
+            eo[mt][e] = E_MIN;
             qf[mt][e] = sm.qf[mt * 8 + 2 * t + e];
             tq[mt][e] = t_first + i0 + row_of(min(m, M - 1) - m0);
         }
@@ -366,57 +403,59 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
         for (int n = 0; n < 2; ++n)
             all_whole = all_whole && there[n] && j0[n] + ROWS <= len && (!a.causal || j0[n] + ROWS - 1 <= t_lo) &&
                         (!a.window || j0[n] > t_hi - a.window || j0[n] + ROWS <= a.sinks);
+        const float lv = log2_floor(fmaxf(vscale[0], vscale[1]));
         // probabilities
         uint32_t ph[MT][2][2], pl[MT][2][2];   // B fragments of P.V: keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of row g
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             uint32_t see = 0xFFu;         // bit 4 n + e: (key g, row 2 t), (g, 2 t + 1), (g + 8, 2 t), (g + 8, 2 t + 1) of page n
-            float mx[2] = {-INFINITY, -INFINITY}, vm[2];
+            float mx[2];
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[mt][n][e] *= qf[mt][e & 1] * kscale[n];
             if (all_whole) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < 2; ++e)
                     mx[e] = fmaxf(fmaxf(c[mt][0][e], c[mt][0][2 + e]), fmaxf(c[mt][1][e], c[mt][1][2 + e]));
-                    vm[e] = fmaxf(vscale[0], vscale[1]);
-                }
             } else {
-                vm[0] = vm[1] = 0.0f;
+                mx[0] = mx[1] = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool y = there[n] && sees(a, tq[mt][e & 1], j0[n] + g + (e >> 1) * 8, len);
-                        if (y) mx[e & 1] = fmaxf(mx[e & 1], c[mt][n][e]);
+                        if (there[n] && sees(a, tq[mt][e & 1], j0[n] + g + (e >> 1) * 8, len)) mx[e & 1] = fmaxf(mx[e & 1], c[mt][n][e]);
                         else see &= ~(1u << (4 * n + e));
-                        // some lane of the row sees a key of this page
-                        if (__ballot_sync(0xffffffffu, y) & (0x11111111u << t)) vm[e & 1] = fmaxf(vm[e & 1], vscale[n]);
                     }
             }
-            if (__any_sync(0xffffffffu, mx[0] > mref[mt][0] + THR || mx[1] > mref[mt][1] + THR ||
-                                            vm[0] > 16.0f * E[mt][0] || vm[1] > 16.0f * E[mt][1])) {
+            if (__any_sync(0xffffffffu, unsettled(mx[0], lv, mref[mt][0], eo[mt][0]) ||
+                                            unsettled(mx[1], lv, mref[mt][1], eo[mt][1]))) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-                    const bool move = mx[e] > mref[mt][e] + THR;
-                    const float mn = move ? mx[e] : mref[mt][e];
-                    const float En = vm[e] > 16.0f * E[mt][e] ? o_unit(vm[e]) : E[mt][e];
-                    const float cl = move ? ex2(mref[mt][e] - mn) : 1.0f, co = cl * (E[mt][e] * inv_pow2(En));
-                    l[mt][e] *= cl;
+                    const float d = move_m(mx[e], mref[mt][e]);
+                    float need = -INFINITY;   // of the keys that this lane's row sees
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float ln = log2_floor(vscale[n]);
+#pragma unroll
+                        for (int h = 0; h < 4; h += 2)
+                            if (see >> (4 * n + h + e) & 1) need = fmaxf(need, fmaxf(c[mt][n][h + e] - mref[mt][e], FAR) + ln);
+                    }
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) need = fmaxf(need, __shfl_xor_sync(0xffffffffu, need, x));
+                    const float co = pow2i(move_e(need, d, eo[mt][e]));
+                    l[mt][e] *= pow2i(fmaxf(d, -127.0f));
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) { o[mt][j][e] *= co; o[mt][j][2 + e] *= co; }
-                    mref[mt][e] = mn;
-                    E[mt][e] = En;
                 }
             }
             float p[2][4], sub[2], vr[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 sub[e] = OFF - (mref[mt][e] == -INFINITY ? 0.0f : mref[mt][e]);
-                vr[e] = inv_pow2(E[mt][e]);
+                vr[e] = pow2i(-eo[mt][e]);
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -525,11 +564,11 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
             const int row = mt * 8 + 2 * t + e;
             if (g == 0) { sm.m[warp][row] = mref[mt][e]; sm.l[warp][row] = x; }
             float *dst = sm.o[warp][row] + g * VB;
+            const float E = pow2i(eo[mt][e]);
 #pragma unroll
             for (int j = 0; j < NJ; j += 2)
                 *reinterpret_cast<float4 *>(dst + 2 * j) =
-                    make_float4(o[mt][j][e] * E[mt][e], o[mt][j][2 + e] * E[mt][e], o[mt][j + 1][e] * E[mt][e],
-                                o[mt][j + 1][2 + e] * E[mt][e]);
+                    make_float4(o[mt][j][e] * E, o[mt][j][2 + e] * E, o[mt][j + 1][e] * E, o[mt][j + 1][2 + e] * E);
         }
     __syncthreads();
     const size_t rows_all = (size_t)a.n_rows * a.heads;

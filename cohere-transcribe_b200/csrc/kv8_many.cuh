@@ -24,7 +24,7 @@
 // swizzle; Q.K reads K that way K-major, P.V reads V MN-major (dims
 // contiguous), so nothing is transposed.  Block scales never touch the
 // operands: K's multiply the scores (one factor per 16 columns), V's the
-// probabilities, relative to a power of two per row that O is held in.
+// probabilities, in units of a power of two per row that O is held in.
 // P [128 x 128] fp16 replaces S in TMEM as the A operand: the 32 columns of 32
 // scores hold their high parts in the first 16 and their low parts in the rest.
 //
@@ -171,8 +171,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
     constexpr bool TWO = sizeof(T) == 4;
     constexpr int TILE = TWO ? 128 : 256;
     constexpr int NB = D / 64;
-    constexpr float THR = TWO ? 4.0f : 8.0f;    // how far a maximum may pass a row's reference unheeded (log2)
-    constexpr float OFF = TWO ? 7.0f : 3.0f;    // P = 2^(x - reference + OFF) vs / 2^e <= 2^(THR + OFF + 4) = 2^15
     constexpr uint32_t COL_S = 0, COL_O = 256;  // S of stream i at 128 i, O at 256 + 128 i
     extern __shared__ __align__(1024) uint8_t many_raw[];
     ManySmem<D> &sm = *reinterpret_cast<ManySmem<D> *>((reinterpret_cast<uintptr_t>(many_raw) + 1023) & ~(uintptr_t)1023);
@@ -411,7 +409,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
         const int t = t_first + i0 + row_of((m < M ? m : M - 1) - m0);
         const int hi = a.causal ? min(len, t + 1) : len;   // sees j < hi and (j >= lo or j < sinks)
         const int lo = a.window ? max(0, t - a.window + 1) : 0;
-        float mref = -INFINITY, l = 0.0f, E = 1.1754944e-38f;   // O is held in units of E, a power of two
+        float mref = -INFINITY, l = 0.0f, eo = E_MIN;      // O is held in units of 2^eo
         bool ok = true;
         const int mine = TWO ? (nt - i + 1) / 2 : nt;      // tiles of this stream
         for (int k = 0; k < mine; ++k) {
@@ -429,31 +427,32 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                 const int j0 = base[b];
                 every = every && j0 + ROWS <= hi && (j0 >= lo || j0 + ROWS <= a.sinks);
             }
-            float mx = -INFINITY, vmax = 0.0f;
+            float mx = -INFINITY, vmax = 0.0f, xb[KB];     // largest score of all, of each block
             float sub, inv;
-            // moves the reference and E when this tile asks for it
+            // moves the reference and the unit when this tile asks for it
             auto settle = [&]() {
-                const bool move = mx > mref + THR;         // always once a first key is seen
-                const float mn = move ? mx : mref;
-                const float En = vmax > 16.0f * E ? o_unit(vmax) : E;
-                if (__any_sync(0xffffffffu, move || En != E)) {
-                    const float cl = move ? ex2(mref - mn) : 1.0f, corr = cl * (E * inv_pow2(En));
-                    l *= cl;
-                    if (k > 0) {
+                const bool look = unsettled(mx, log2_floor(vmax), mref, eo);
+                if (__any_sync(0xffffffffu, look)) {
+                    const float d = move_m(mx, mref);
+                    float need = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+                        if (xb[b] != -INFINITY) need = fmaxf(need, fmaxf(xb[b] - mref, FAR) + log2_floor(vs[b]));
+                    const float co = pow2i(move_e(need, d, eo));
+                    l *= pow2i(fmaxf(d, -127.0f));
+                    if (k > 0 && __any_sync(0xffffffffu, co != 1.0f)) {
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             float o[32];
                             tmem_ld32(to + 32 * c, o);
 #pragma unroll
-                            for (int q = 0; q < 32; ++q) o[q] *= corr;
+                            for (int q = 0; q < 32; ++q) o[q] *= co;
                             tmem_store32(to + 32 * c, o);
                         }
                     }
-                    mref = mn;
-                    E = En;
                 }
                 sub = OFF - (mref == -INFINITY ? 0.0f : mref);
-                inv = inv_pow2(E);
+                inv = pow2i(-eo);
             };
             auto pack = [&](const float *v, int c) {       // 32 probabilities -> TMEM, over their scores
                 uint32_t phi[16], plo[16];
@@ -490,7 +489,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                     for (int q = 0; q < 4; ++q)
                         bm[q] = fmaxf(fmaxf(v[16 * b + q], v[16 * b + 4 + q]), fmaxf(v[16 * b + 8 + q], v[16 * b + 12 + q]));
                     const float x = fmaxf(fmaxf(bm[0], bm[1]), fmaxf(bm[2], bm[3])) * (rf * ks[b]);
+                    xb[b] = -INFINITY;
                     if (!MASKED || see) {
+                        xb[b] = x;
                         mx = fmaxf(mx, x);
                         vmax = fmaxf(vmax, vs[b]);
                     }
@@ -537,18 +538,18 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                 }
                 sm.join[0][ql] = mref;
                 sm.join[1][ql] = l;
-                sm.join[2][ql] = E;
+                sm.join[2][ql] = eo;
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
         }
         if (ok && (!TWO || i == 0)) {
-            float f0 = E, f1 = 0.0f;
+            float f0 = pow2i(eo), f1 = 0.0f;
             if (TWO && nt > 1) {
                 const float m1 = sm.join[0][ql], mn = fmaxf(mref, m1), ref = mn == -INFINITY ? 0.0f : mn;
                 const float c0 = ex2(mref - ref), c1 = ex2(m1 - ref);
                 l = l * c0 + sm.join[1][ql] * c1;
-                f0 = E * c0;
-                f1 = sm.join[2][ql] * c1;
+                f0 *= c0;
+                f1 = pow2i(sm.join[2][ql]) * c1;
                 mref = mn;
             }
             const bool store = m < M;

@@ -381,6 +381,70 @@ def test_attention_uneven_block_scales(kv8, torch, typ, rows):
     check_attend(kv8, c, s, rc, table, lens, [rows] * 2, 6, typ)
 
 
+def row_bounds(rc, layer, table, lens, q, starts, scale, causal, window, sinks, typ):
+    """Attention in 64 bits, and what its rounding errors may add up to when each key's are counted by what the key adds
+    (reach, masses and sums as above, but none of them may be excused by a key that a row hardly feels):
+      a probability is off by at most dx of its own key, relative: sum_j p_j dx_j (|v_j| + |out|);
+      its fp16 form by 2^-22 (one fp16: 2^-11), and the sums by (pages + 64) 2^-22, relative to mass;
+      an fp16's absolute step 2^-24, that is 2^-25 an entry, counts in units of which the row's largest product of
+      probability and V scale is at least 2^8: 2^-33 max_j(p_j scale_j) sum |code|."""
+    import torch
+    R, H, D = q.shape
+    G, pages = H // rc.v.shape[3], max(len(r) for r in table)
+    out, tol = np.zeros((R, H, D)), np.zeros((R, H, D))
+    for s, L in enumerate(lens):
+        n, rows = starts[s + 1] - starts[s], slice(starts[s], starts[s + 1])
+        row = table[s][:ref.pages_of(L)]
+        t, j = L - n + np.arange(n)[:, None], np.arange(L)[None]
+        see = np.broadcast_to(ref.sees(t, j, L, causal, window, sinks), (n, L))
+        for h in range(H):
+            K, V = rc.rows(layer, row, L, h // G)
+            unit = np.repeat(rc.s[row, layer, 1, h // G], ROWS)[:L]
+            code = np.abs(rc.v[row, layer, 1, h // G].reshape(-1, D)[:L])
+            x = np.where(see, scale * (q[rows, h] @ K.T), -np.inf)
+            p = np.exp(x - x.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            reach = scale * np.abs(q[rows, h]).max(1, keepdims=True) * np.abs(K).sum(1)
+            dx = 1.1 * (reach * (D / 16 + 10) * 2.0 ** -22 + 2.0 ** -20)
+            o, mass = p @ V, p @ np.abs(V)
+            rel = (2.0 ** -11 if typ == "bfloat16" else 2.0 ** -22) + (pages + 64) * 2.0 ** -22
+            out[rows, h] = o
+            tol[rows, h] = ((p * dx) @ np.abs(V) + (p * dx).sum(1, keepdims=True) * np.abs(o) + mass * rel
+                            + 2.0 ** -33 * (p * unit).max(1, keepdims=True) * (see @ code)
+                            + np.abs(o) * (torch.finfo(getattr(torch, typ)).eps / 2) + 1e-37)
+    return out, tol
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,heads", [(1, 2), (1, 8), (5, 12), (150, 4)])
+@pytest.mark.parametrize("place", ["first", "last", "spread"])
+def test_attention_value_scales_far_apart(kv8, torch, fmt, typ, rows, heads, place):
+    """Blocks whose V scale is 2^k times the others' and whose probability is 2^-k of theirs, or next to nothing:
+    the others keep their bits."""
+    dim, kvh, n = 64, 2, 600
+    lens, st = [n + rows, 200 + rows], [0, rows, 2 * rows]
+    for k in (10, 20, 30, 40):
+        for drop in (k, 200):
+            c, s, rc, table = make(kv8, fmt, lens, kvh, dim, seed=k + drop)
+            gen = torch.Generator(device="cuda").manual_seed(k)
+            q = (torch.randn(2 * rows, heads, dim, device="cuda", generator=gen).abs() + 0.5).to(getattr(torch, typ))
+            for i, L in enumerate(lens):
+                big = {"first": range(0, 9), "last": range(L // ROWS - 4, L // ROWS), "spread": range(1, L // ROWS, 3)}[place]
+                for b in big:
+                    page = table[i][b]
+                    # K rows of -1 times a factor: q's mean entry is about 1.3, so a score falls by 0.125 * 64 * 1.3 of it
+                    c.codes[page, 1, 0] = 0xB8 if fmt == "e4m3" else 0xFF              # -1
+                    c.scales[page, 1, 0] = drop * math.log(2) / (0.125 * 64 * 1.3)
+                    c.scales[page, 1, 1] *= 2.0 ** k
+            rc = ref.Cache(to_values(c.codes, fmt), c.scales.cpu().numpy().astype(np.float64), rc.refs, fmt)
+            got = c.attend(1, s, q, row_start=dev(st), max_rows=rows).double().cpu().numpy()
+            want, tol = row_bounds(rc, 1, table, lens, q.double().cpu().numpy(), st, 0.125, True, 0, 0, typ)
+            assert c.status() == 0
+            worst = np.abs(got - want) / tol
+            assert (worst <= 1).all(), (k, drop, float(np.nanmax(worst)), float(np.abs(got - want).max()))
+
+
 def test_attention_extreme_queries(kv8, torch):
     """Very large and very small queries, and a scale that makes one key take all."""
     lens = [90, 40]
