@@ -913,7 +913,7 @@ extern "C" int ct_kv8_compact(const ct_kv8_cache *c, const ct_kv8_seqs *s, int *
 }
 
 extern "C" int ct_kv8_copy_pages(const ct_kv8_cache *c, const int *src, const int *dst, int n, void *stream) {
-    if (!good_cache(c) || !src || !dst || n < 0 || n > 4096) return CT_EINVAL;
+    if (!good_cache(c) || n < 0 || n > 4096 || (n && (!src || !dst))) return CT_EINVAL;
     if (cudaPeekAtLastError() != cudaSuccess) return CT_EDEVICE;
     if (n == 0) return CT_OK;
     const Pool p = pool_of(c);

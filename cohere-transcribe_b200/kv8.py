@@ -212,7 +212,10 @@ class Cache:
     def free(self, seqs, which=None):
         """Release all sequences, or those listed in which (ct_kv8_free)."""
         w = None if which is None else _ints(which, None, self.device, "which")
-        self._call("ct_kv8_free", self.ref, self._seqs(seqs), w, 0 if which is None else which.numel())
+        p = self._seqs(seqs)
+        if which is not None and which.numel() == 0:   # its address is NULL, which means all
+            return
+        self._call("ct_kv8_free", self.ref, p, w, 0 if which is None else which.numel())
 
     def trim(self, seqs, window, sinks=0):
         """Release the pages that a window has passed (ct_kv8_trim)."""

@@ -641,6 +641,15 @@ def test_free_and_its_indices(kv8):
     c.free(s, dev([]).int())
 
 
+def test_empty_lists_do_nothing(kv8, torch):
+    """An empty list of sequences or pages is not the C interface's NULL, which means all."""
+    c, s, table, lens, refs = pool(kv8, 400, 50, 9, 5)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    c.free(s, none)
+    c.copy_pages(none, none)
+    assert c.status() == 0 and s.lens.tolist() == lens and c.refs.tolist() == refs
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (40, 4), (16, 16), (33, 17), (10000, 0), (5, 10000)])
 def test_trim(kv8, window, sinks):
     c, s, table, lens, refs = pool(kv8, 400, 50, 9, 6)
