@@ -407,8 +407,12 @@ __global__ void __launch_bounds__(128) free_kernel(const Pool p, const int *tabl
         return;
     }
     if (threadIdx.x == 0) {
-        sm_len = atomicExch(&len[s], 0);   // an index listed twice finds 0 the second time
-        if (sm_len > stride * ROWS) { set_status(CT_STATUS_BAD_ARG); sm_len = stride * ROWS; }
+        if (len[s] > stride * ROWS) {      // what its row holds is not all its own
+            set_status(CT_STATUS_BAD_ARG);
+            sm_len = 0;
+        } else {
+            sm_len = atomicExch(&len[s], 0);   // an index listed twice finds 0 the second time
+        }
     }
     __syncthreads();
     const int n = pages_of(max(sm_len, 0));
@@ -418,7 +422,11 @@ __global__ void __launch_bounds__(128) free_kernel(const Pool p, const int *tabl
 __global__ void __launch_bounds__(128) trim_kernel(const Pool p, int *table, const int *len, int stride, int window,
                                                    int sinks) {
     const int s = blockIdx.x;
-    const int n = min(len[s], stride * ROWS);
+    const int n = len[s];
+    if (n > stride * ROWS) {
+        if (threadIdx.x == 0) set_status(CT_STATUS_BAD_ARG);
+        return;
+    }
     const int end = n > window ? (n - window) / ROWS : 0;
     for (int j = pages_of(sinks) + threadIdx.x; j < end; j += 128) {
         int *e = table + (size_t)s * stride + j;
@@ -529,7 +537,12 @@ __global__ void __launch_bounds__(256) compact_kernel(const CompactArgs a, int s
         if (a.rank[p] == -1) a.refs_out[p] = a.p.refs[p];
     for (long long e = t0; e < (long long)a.n * a.stride; e += step) {
         const int s = (int)(e / a.stride), j = (int)(e % a.stride);
-        if (j >= pages_of(max(a.len[s], 0))) continue;
+        const int len = a.len[s];
+        if (len > a.stride * ROWS) {
+            if (j == 0) set_status(CT_STATUS_BAD_ARG);
+            continue;
+        }
+        if (j >= pages_of(max(len, 0))) continue;
         const int p = a.table[e];
         int to = p;
         if (p != -1 && !a.p.has(p)) set_status(CT_STATUS_BAD_ARG);

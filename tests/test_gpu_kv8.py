@@ -641,6 +641,39 @@ def test_free_and_its_indices(kv8):
     c.free(s, dev([]).int())
 
 
+@pytest.mark.parametrize("length", [9 * ROWS + 1, 2 ** 30 + 1, 2 ** 31 - 16, 2 ** 31 - 1])
+def test_page_operators_leave_out_lengths_beyond_the_table(kv8, torch, length):
+    """Such a sequence stays as it is (status); the others are served."""
+    def start():
+        c, s, table, lens, refs = pool(kv8, 400, 20, 9, 5, share=False)
+        s.lens[7] = length
+        s.table[7] = torch.arange(9, dtype=torch.int32, device="cuda")     # whatever lies there is not its own
+        table[7] = list(range(9))
+        return c, s, table, lens[:7] + [length] + lens[8:], refs
+
+    c, s, table, lens, refs = start()
+    ref.release(table, lens, refs, [i for i in range(20) if i != 7])
+    c.free(s)
+    assert c.status() == BAD_ARG and s.lens.tolist() == lens and c.refs.tolist() == refs
+    c.free(s, dev([7, 7]))
+    assert c.status() == BAD_ARG and s.lens.tolist() == lens and c.refs.tolist() == refs
+
+    c, s, table, lens, refs = start()
+    short = lens[:7] + [0] + lens[8:]
+    ref.trim(table, short, refs, 20, 0)
+    c.trim(s, 20, 0)
+    assert c.status() == BAD_ARG and s.table.tolist() == table and c.refs.tolist() == refs and s.lens.tolist() == lens
+
+    c, s, table, lens, refs = start()
+    new_table, new_refs, _, _ = ref.compact(table, lens[:7] + [0] + lens[8:], refs)
+    c.compact(s)
+    assert c.status() == BAD_ARG and s.table.tolist() == new_table and c.refs.tolist() == new_refs
+
+    c, s, table, lens, refs = start()
+    c.reserve(s, dev([0] * 7 + [5] + [0] * 12))
+    assert c.status() == BAD_ARG and s.table.tolist() == table and c.refs.tolist() == refs and s.lens.tolist() == lens
+
+
 def test_empty_lists_do_nothing(kv8, torch):
     """An empty list of sequences or pages is not the C interface's NULL, which means all."""
     c, s, table, lens, refs = pool(kv8, 400, 50, 9, 5)
