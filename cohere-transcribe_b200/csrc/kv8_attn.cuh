@@ -564,11 +564,13 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
             const int row = mt * 8 + 2 * t + e;
             if (g == 0) { sm.m[warp][row] = mref[mt][e]; sm.l[warp][row] = x; }
             float *dst = sm.o[warp][row] + g * VB;
-            const float E = pow2i(eo[mt][e]);
+            // each warp's own mean of V: no sum of values can overflow (nor 2^eo / l underflow)
+            const float inv = x == 0.0f ? 0.0f : 1.0f / x, E = pow2i(eo[mt][e]);
 #pragma unroll
             for (int j = 0; j < NJ; j += 2)
                 *reinterpret_cast<float4 *>(dst + 2 * j) =
-                    make_float4(o[mt][j][e] * E, o[mt][j][2 + e] * E, o[mt][j + 1][e] * E, o[mt][j + 1][2 + e] * E);
+                    make_float4(o[mt][j][e] * inv * E, o[mt][j][2 + e] * inv * E, o[mt][j + 1][e] * inv * E,
+                                o[mt][j + 1][2 + e] * inv * E);
         }
     __syncthreads();
     const size_t rows_all = (size_t)a.n_rows * a.heads;
@@ -579,12 +581,14 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
 #pragma unroll
         for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm.m[w][row]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
-        float lsum = 0.0f;
+        float lw[4], lsum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) lsum += lw[w] = sm.l[w][row] * ex2(sm.m[w][row] - ref);
+        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;       // a row that sees nothing: zeros
         float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = ex2(sm.m[w][row] - ref);
-            lsum += sm.l[w][row] * f;
+            const float f = lw[w] * inv;
             const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][row][d]);
             acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
         }
@@ -596,9 +600,7 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
         const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
         const size_t r = (size_t)sp.first + i0 + qi;
         if (pieces == 1) {
-            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;   // a row that sees nothing: zeros
-            store4(static_cast<T *>(a.out) + r * a.ldo + (size_t)h * D + d, acc.x * inv, acc.y * inv, acc.z * inv,
-                   acc.w * inv);
+            store4(static_cast<T *>(a.out) + r * a.ldo + (size_t)h * D + d, acc.x, acc.y, acc.z, acc.w);
         } else {
             const size_t b = (r * a.heads + h) * a.max_chunks + piece;
             *reinterpret_cast<float4 *>(a.part + b * D + d) = acc;
@@ -611,28 +613,37 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     for (int i = piece * 128 + threadIdx.x; i < 8 * MT * (D / 4); i += a.max_chunks * 128) {
         const int row = i / (D / 4), d = (i % (D / 4)) * 4;
         if (m0 + row >= M) break;
-        float mx = -INFINITY;
-        for (int c = 0; c < pieces; ++c) mx = fmaxf(mx, dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].x), c)));
+        float mc[8], lc[8], mx = -INFINITY, lsum = 0.0f;           // a cluster has 8 pieces at most
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < pieces) {
+                mc[c] = dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].x), c));
+                lc[c] = dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].y), c));
+                mx = fmaxf(mx, mc[c]);
+            }
         const float ref = mx == -INFINITY ? 0.0f : mx;
-        float lsum = 0.0f;
-        float4 acc = make_float4(0, 0, 0, 0);
-        for (int c = 0; c < pieces; ++c) {
-            const float f = ex2(dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].x), c)) - ref);
-            lsum += dsmem_ld(dsmem_addr(smem_u32(&sm.ml[row].y), c)) * f;
-            const float4 x = dsmem_ld4(dsmem_addr(smem_u32(&sm.o[0][row][d]), c));
-            acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-        }
-        const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < pieces) lsum += lc[c] *= ex2(mc[c] - ref);
         const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-        store4(static_cast<T *>(a.out) + ((size_t)sp.first + i0 + qi) * a.ldo + (size_t)h * D + d, acc.x * inv, acc.y * inv,
-               acc.z * inv, acc.w * inv);
+        float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c < pieces) {
+                const float f = lc[c] * inv;
+                const float4 x = dsmem_ld4(dsmem_addr(smem_u32(&sm.o[0][row][d]), c));
+                acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+            }
+        const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
+        store4(static_cast<T *>(a.out) + ((size_t)sp.first + i0 + qi) * a.ldo + (size_t)h * D + d, acc.x, acc.y, acc.z, acc.w);
     }
     cluster_sync();                       // nobody leaves while its results are being read
 }
 
-// Joins the pieces of each row: a warp per row, pieces in order, eight loads in
-// flight (3 us for 512 rows of two pieces; launch latency is hidden behind the
-// kernel before it).
+// Joins the pieces of each row, each of them the mean of its own V rows with the
+// reference m and the sum l of its probabilities, by weights that add up to 1: a warp
+// per row, pieces in order, eight loads in flight (3 us for 512 rows of two pieces;
+// launch latency is hidden behind the kernel before it).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, int tile_rows) {
     pdl_wait();
@@ -656,25 +667,26 @@ __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, int tile_ro
         mx = warp_max(mx);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float l = 0.0f, acc[W];
+        for (int c = lane; c < pieces; c += 32) l += ml[c].y * ex2(ml[c].x - ref);
+        l = warp_sum(l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int i = 0; i < W; ++i) acc[i] = 0.0f;
 #pragma unroll 8
         for (int c = 0; c < pieces; ++c) {
             const float2 x = ml[c];
-            const float f = ex2(x.x - ref);
-            l += x.y * f;
+            const float f = x.y * ex2(x.x - ref) * inv;
             const float *src = a.part + (b + c) * D + lane * W;
 #pragma unroll
             for (int i = 0; i < W; ++i) acc[i] = fmaf(src[i], f, acc[i]);
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T *dst = static_cast<T *>(a.out) + r * a.ldo + (size_t)h * D + lane * W;
         if (W == 4) {
-            store4(dst, acc[0] * inv, acc[1] * inv, acc[W - 2] * inv, acc[W - 1] * inv);
+            store4(dst, acc[0], acc[1], acc[W - 2], acc[W - 1]);
         } else if (sizeof(T) == 4) {
-            *reinterpret_cast<float2 *>(dst) = make_float2(acc[0] * inv, acc[1] * inv);
+            *reinterpret_cast<float2 *>(dst) = make_float2(acc[0], acc[1]);
         } else {
-            *reinterpret_cast<__nv_bfloat162 *>(dst) = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+            *reinterpret_cast<__nv_bfloat162 *>(dst) = __floats2bfloat162_rn(acc[0], acc[1]);
         }
     }
 }

@@ -543,23 +543,24 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
             asm volatile("bar.sync 1, 256;" ::: "memory");
         }
         if (ok && (!TWO || i == 0)) {
-            float f0 = pow2i(eo), f1 = 0.0f;
+            // The mean of this piece's V, not their sum: O / l first, then the unit, so that
+            // neither the values' sum overflows nor 2^eo / l underflows.
+            float f0 = 1.0f, f1 = 0.0f, e1 = 0.0f;
+            const float e0 = pow2i(eo);
             if (TWO && nt > 1) {
                 const float m1 = sm.join[0][ql], mn = fmaxf(mref, m1), ref = mn == -INFINITY ? 0.0f : mn;
-                const float c0 = ex2(mref - ref), c1 = ex2(m1 - ref);
-                l = l * c0 + sm.join[1][ql] * c1;
-                f0 *= c0;
-                f1 = pow2i(sm.join[2][ql]) * c1;
+                f0 = ex2(mref - ref);
+                f1 = ex2(m1 - ref);
+                l = l * f0 + sm.join[1][ql] * f1;
+                e1 = pow2i(sm.join[2][ql]);
                 mref = mn;
             }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // a row that sees nothing: zeros
+            f0 *= inv;
+            f1 *= inv;
             const bool store = m < M;
             const int q = row_of(r), h = hk * G + g0 + r - q * G;
             const size_t row = (size_t)sp.first + (store ? i0 + q : 0);
-            if (pieces == 1) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing: zeros
-                f0 *= inv;
-                f1 *= inv;
-            }
             T *dst = static_cast<T *>(a.out) + row * a.ldo + (size_t)h * D;
             const size_t b = (row * a.heads + h) * a.max_chunks + piece;
 #pragma unroll 1
@@ -568,8 +569,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
                 tmem_ld32(to + 32 * c, v);
 #pragma unroll
                 for (int q = 0; q < 32; ++q) {
-                    v[q] *= f0;
-                    if (TWO && nt > 1) v[q] = fmaf(oj[(32 * c + q) * 128 + ql], f1, v[q]);
+                    v[q] = v[q] * f0 * e0;
+                    if (TWO && nt > 1) v[q] = fmaf(oj[(32 * c + q) * 128 + ql] * f1, e1, v[q]);
                 }
                 if (store) {
 #pragma unroll

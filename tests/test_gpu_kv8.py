@@ -381,7 +381,7 @@ def test_attention_uneven_block_scales(kv8, torch, typ, rows):
     check_attend(kv8, c, s, rc, table, lens, [rows] * 2, 6, typ)
 
 
-def row_bounds(rc, layer, table, lens, q, starts, scale, causal, window, sinks, typ):
+def row_bounds(rc, layer, table, lens, q, starts, scale, causal, window, sinks, typ, tiny=1e-37):
     """Attention in 64 bits, and what its rounding errors may add up to when each key's are counted by what the key adds
     (reach, masses and sums as above, but none of them may be excused by a key that a row hardly feels):
       a probability is off by at most dx of its own key, relative: sum_j p_j dx_j (|v_j| + |out|);
@@ -411,7 +411,7 @@ def row_bounds(rc, layer, table, lens, q, starts, scale, causal, window, sinks, 
             out[rows, h] = o
             tol[rows, h] = ((p * dx) @ np.abs(V) + (p * dx).sum(1, keepdims=True) * np.abs(o) + mass * rel
                             + 2.0 ** -33 * (p * unit).max(1, keepdims=True) * (see @ code)
-                            + np.abs(o) * (torch.finfo(getattr(torch, typ)).eps / 2) + 1e-37)
+                            + np.abs(o) * (torch.finfo(getattr(torch, typ)).eps / 2) + tiny)
     return out, tol
 
 
@@ -443,6 +443,29 @@ def test_attention_value_scales_far_apart(kv8, torch, fmt, typ, rows, heads, pla
             assert c.status() == 0
             worst = np.abs(got - want) / tol
             assert (worst <= 1).all(), (k, drop, float(np.nanmax(worst)), float(np.abs(got - want).max()))
+
+
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("size", [2e38, 1e37, 1e-36])
+@pytest.mark.parametrize("rows,past,heads", [(1, 40, 2), (1, 700, 2), (1, 6000, 8), (3, 3000, 10), (150, 20, 4), (150, 3000, 4)])
+def test_attention_of_values_near_the_ends_of_fp32(kv8, torch, typ, size, rows, past, heads):
+    """A result lies between the values it is made of: it overflows nowhere on its way, and small ones keep their
+    bits. One row and several, one piece, a cluster's pieces and those that a second kernel joins."""
+    kvh, dim = 2, 64
+    lens, st = [past + rows, past // 2 + rows], [0, rows, 2 * rows]
+    c, s, rc, table = make(kv8, "e4m3", lens, kvh, dim)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    kv = [torch.rand(sum(lens), kvh, dim, device="cuda", generator=gen) - 0.5 for _ in range(2)]
+    c.append(1, s, kv[0], kv[1] * size * 2, row_start=dev(starts_of(lens)), max_rows=max(lens))
+    q = torch.randn(2 * rows, heads, dim, device="cuda", generator=gen).to(getattr(torch, typ))
+    rc = ref.Cache(to_values(c.codes, "e4m3"), c.scales.cpu().numpy().astype(np.float64), rc.refs, "e4m3")
+    got = c.attend(1, s, q, row_start=dev(st), max_rows=rows).double().cpu().numpy()
+    # below the smallest normal number, 2^-126, a product's step is 2^-149 (a few of them), and the type's own 2^-126 eps
+    tiny = 2.0 ** -146 + 2.0 ** -126 * torch.finfo(getattr(torch, typ)).eps / 2
+    want, tol = row_bounds(rc, 1, table, lens, q.double().cpu().numpy(), st, 0.125, True, 0, 0, typ, tiny=tiny)
+    assert c.status() == 0 and np.isfinite(want.astype(np.float32)).all()
+    worst = np.abs(got - want) / tol
+    assert (worst <= 1).all(), (float(np.nanmax(worst)), int((~np.isfinite(got)).sum()))
 
 
 def test_attention_extreme_queries(kv8, torch):
