@@ -75,10 +75,11 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
 }
 
 // The power of two that brings the largest magnitude of a row into [1, 2); 1 for
-// zero and non-finite ones.
+// zero and subnormal ones, NaN for an infinity: a softmax over scores of +-inf or
+// NaN is NaN, also where all of them are -inf, which else hides a key.
 __device__ __forceinline__ float row_pow2(float amax) {
     const int e = (int)(__float_as_uint(amax) >> 23);
-    return (e == 0 || e == 255) ? 1.0f : __uint_as_float((uint32_t)min(max(254 - e, 1), 253) << 23);
+    return e == 0 ? 1.0f : __uint_as_float(e == 255 ? 0x7FC00000u : (uint32_t)min(max(254 - e, 1), 253) << 23);
 }
 // 1 / x of a power of two in [2^-126, 2^126], without a division.
 __device__ __forceinline__ float inv_pow2(float x) { return __uint_as_float(0x7F000000u - __float_as_uint(x)); }

@@ -446,6 +446,26 @@ def test_attention_value_scales_far_apart(kv8, torch, fmt, typ, rows, heads, pla
 
 
 @pytest.mark.parametrize("typ", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,past", [(1, 1), (1, 700), (3, 40), (150, 20), (150, 2000)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_attention_nonfinite_queries(kv8, torch, typ, rows, past, value):
+    """A row whose query holds an infinity or a NaN is NaN, as its softmax is, whatever the signs in K; the other rows and
+    heads do not feel it, and a row that sees nothing stays zero."""
+    lens, st = [past + rows, rows - 1], [0, rows, 2 * rows]
+    c, s, rc, table = make(kv8, "int8", lens, 2, 64)
+    c.codes[:, 1, 0, 0, :, 3] = 0xFF if value > 0 else 1       # every K of kv head 0 has -1 (or 1) there
+    q = torch.randn(2 * rows, 4, 64, device="cuda").to(getattr(torch, typ))
+    want = c.attend(1, s, q, row_start=dev(st), max_rows=rows)
+    q[0, 1, 3] = q[rows - 1, 0, 3] = q[rows, 1, 3] = value
+    got = c.attend(1, s, q, row_start=dev(st), max_rows=rows)
+    assert c.status() == 0
+    hit = torch.zeros(2 * rows, 4, dtype=torch.bool, device="cuda")
+    hit[0, 1] = hit[rows - 1, 0] = True
+    assert bool(got[hit].isnan().all()) and bool((got[rows] == 0).all())     # row `rows` is before its first token row
+    assert torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("typ", ["float32", "bfloat16"])
 @pytest.mark.parametrize("size", [2e38, 1e37, 1e-36])
 @pytest.mark.parametrize("rows,past,heads", [(1, 40, 2), (1, 700, 2), (1, 6000, 8), (3, 3000, 10), (150, 20, 4), (150, 3000, 4)])
 def test_attention_of_values_near_the_ends_of_fp32(kv8, torch, typ, size, rows, past, heads):
