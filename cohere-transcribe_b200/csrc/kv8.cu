@@ -699,6 +699,10 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
         // bits than 1e-6 and 1.5 times torch's fp32 products, with pieces of 2048 keys
         // 24 of 1412 (4 prompts of 1000 to 4097 rows take 2605 us instead of 2066).
         if (type == CT_KV8_F32 && list > 80) pieces = std::max(pieces, std::min(16ll, (list + 63) / 64));
+        // However long the cache, 16,384 keys a piece (bf16 results 65,536): a step loses
+        // up to 2^-22 of a sum, so 2^-12 (2^-10) of it at most.
+        const long long most = type == CT_KV8_F32 ? 1024 : 4096;
+        pieces = std::max(pieces, (list + most - 1) / most);
         chunk = ((list + pieces - 1) / pieces + KB - 1) / KB * KB;
     }
     pl.chunk = (int)chunk;

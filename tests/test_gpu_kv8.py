@@ -560,6 +560,26 @@ def test_attention_on_two_streams(kv8, torch, rows):
     assert c.status() == 0
 
 
+@pytest.mark.parametrize("typ,pages_a_piece", [("float32", 1024), ("bfloat16", 4096)])
+def test_attention_sums_of_millions_of_keys(kv8, torch, typ, pages_a_piece):
+    """33 rows of each of 148 sequences over the same 16.8 million keys: the sums are cut into pieces however long the
+    cache. All scores are 0, so a result is the mean of V.  The tensor core truncates each of its sums, one per page of a
+    piece, by less than 2^-22 of it; 64 such steps more for the rest, as in the other tests, and half a step of the type."""
+    n, seqs, rows = 1 << 20, 148, 33
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    c = kv8.Cache(torch.zeros(n, 1, 2, 1, ROWS, 64, dtype=torch.uint8, device="cuda"),
+                  torch.full((n, 1, 2, 1), 2.0 ** -6, device="cuda"), None, "int8")
+    c.codes[:, 0, 1] = torch.randint(60, 128, (n, 1, ROWS, 64), dtype=torch.uint8, device="cuda", generator=gen)
+    want = c.codes[:, 0, 1].sum((0, 1, 2), dtype=torch.int64).double() / (n * ROWS * 64)
+    s = kv8.Seqs(torch.arange(n, dtype=torch.int32, device="cuda").expand(seqs, n).contiguous(), dev([n * ROWS] * seqs))
+    q = torch.randn(seqs * rows, 1, 64, device="cuda", generator=gen).to(getattr(torch, typ))
+    out = c.attend(0, s, q, row_start=dev([rows * i for i in range(seqs + 1)]), max_rows=rows, causal=False)
+    assert c.status() == 0
+    tol = want * ((pages_a_piece + 64) * 2.0 ** -22 + torch.finfo(q.dtype).eps / 2)
+    worst = ((out[:, 0].double() - want).abs() / tol).max().item()
+    assert worst <= 1, worst
+
+
 def test_offsets_beyond_32_bits(kv8, torch):
     """Pages whose byte offsets pass 2^32: written, read, copied and moved there."""
     pages, layers, kvh, dim = 20000, 4, 16, 128      # 256 KB each: 5.2 GB
