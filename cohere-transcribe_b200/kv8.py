@@ -38,6 +38,12 @@ def _need(cond, what):
         raise ValueError(what)
 
 
+def _int32(*numbers):
+    """ctypes would cut them to 32 bits without a word."""
+    if max(numbers) > 0x7FFFFFFF or min(numbers) < -0x80000000:
+        raise ValueError("row counts, lengths, windows and sinks: 32-bit integers")
+
+
 def _ints(t, shape, device, what):
     if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_contiguous() and t.device == device
             and (shape is None or t.shape == shape)):
@@ -124,10 +130,10 @@ class Cache:
         if n == 1:
             ld = h * d
         p = x.data_ptr()
-        if (d != self.head_dim or n == 0 or h == 0 or sd != 1 or (sh != d and h > 1) or ld < h * d
+        if (d != self.head_dim or n == 0 or h == 0 or sd != 1 or (sh != d and h > 1) or not h * d <= ld < 1 << 31
                 or x.dtype not in _TYPES or x.device != self.device or (p | ld * x.element_size()) & 15):
             raise ValueError(f"{what}: float32 or bfloat16 [rows, heads, {self.head_dim}] on {self.device}, each row "
-                             "contiguous, rows of 16-byte alignment that do not overlap")
+                             "contiguous, rows of 16-byte alignment that do not overlap, less than 2^31 elements apart")
         return n, h, ld, p
 
     def _ws(self, ws, need):
@@ -155,14 +161,17 @@ class Cache:
         _need(k.dtype == v.dtype and n == nv and h == hv == self.kv_heads,
               f"k and v: the same type and number of rows, {self.kv_heads} heads")
         rs = self._starts(seqs, n, row_start, max_rows)
+        _int32(max_rows)
         self._call("ct_kv8_append", self.ref, self._layer(layer), self._seqs(seqs), pk, ldk, pv, ldv,
                    _TYPES[k.dtype], n, rs, max_rows)
 
     def attend_workspace(self, seqs, q, max_rows=1, max_len=None, causal=True, window=0, sinks=0):
         """A workspace for `attend` calls of these sizes (one per stream that may run them at the same time)."""
         n, h, _, _ = self._rows(q, "q")
-        n = self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, _TYPES[q.dtype], n, max_rows,
-                                          seqs.max_pages * ROWS if max_len is None else max_len, h, int(causal),
+        if max_len is None:
+            max_len = seqs.max_pages * ROWS
+        _int32(max_rows, max_len, window, sinks)
+        n = self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, _TYPES[q.dtype], n, max_rows, max_len, h, int(causal),
                                           window, sinks)
         return torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
 
@@ -182,6 +191,7 @@ class Cache:
         rs = self._starts(seqs, n, row_start, max_rows)
         if max_len is None:
             max_len = seqs.max_pages * ROWS
+        _int32(max_rows, max_len, window, sinks)
         causal = int(causal)
         ws, pw, nw = self._ws(ws, lambda: self.lib.ct_kv8_attn_ws_bytes(self.ref, seqs.ref, typ, n, max_rows, max_len,
                                                                        h, causal, window, sinks))
@@ -219,6 +229,7 @@ class Cache:
 
     def trim(self, seqs, window, sinks=0):
         """Release the pages that a window has passed (ct_kv8_trim)."""
+        _int32(window, sinks)
         self._call("ct_kv8_trim", self.ref, self._seqs(seqs), window, sinks)
 
     def compact(self, seqs, refs_out=None, table_out=None, n_live=None, ws=None):

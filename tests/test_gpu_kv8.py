@@ -829,6 +829,25 @@ def test_python_checks_arguments(kv8, torch):
         assert e.value.code == -1
 
 
+def test_python_refuses_numbers_beyond_32_bits(kv8, torch):
+    """The C interface takes 32-bit integers: 2^32 must not arrive as 0, nor a row stride lose its top."""
+    c, s, *_ = make(kv8, "int8", [400, 20], 1, 64)
+    q, big = torch.randn(2, 1, 64, device="cuda"), 1 << 32
+    refs, table = c.refs.clone(), s.table.clone()
+    far = torch.empty_strided((2, 1, 64), (big + 64, 64, 1), dtype=torch.bfloat16, device="cuda")
+    st = dev([0, 1, 2])
+    bad = [lambda: c.attend(0, s, q, window=big), lambda: c.attend(0, s, q, window=16, sinks=big + 1),
+           lambda: c.attend(0, s, q, max_len=big + 400), lambda: c.attend(0, s, q, row_start=st, max_rows=big + 1),
+           lambda: c.attend(0, s, q, window=-big), lambda: c.attend(0, s, far), lambda: c.append(0, s, far, far),
+           lambda: c.append(0, s, q, q, row_start=st, max_rows=big + 1), lambda: c.attend_workspace(s, q, max_len=big + 400),
+           lambda: c.trim(s, big + 1), lambda: c.trim(s, 16, big)]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was taken")
+    assert c.status() == 0 and torch.equal(c.refs, refs) and torch.equal(s.table, table)
+
+
 def test_python_refuses_a_misaligned_pool(kv8, torch):
     arena = torch.zeros(2 * 2 * ROWS * 64 + 16, dtype=torch.uint8, device="cuda")
     scales = torch.zeros(2, 1, 2, 1, device="cuda")
