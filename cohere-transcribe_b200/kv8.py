@@ -2,7 +2,7 @@
 
 `Cache` and `Seqs` hold the tensors a caller owns; the methods check their
 arguments and call the C entry points on the current torch stream of the
-cache's device.  They never synchronise (`status` does).
+cache's device.  They never synchronise (`status` does, and `values` without `n`).
 
     cache = Cache.empty(n_pages, n_layers, kv_heads, head_dim, "e4m3")
     seqs = Seqs.empty(n_seqs, max_pages)
@@ -255,9 +255,13 @@ class Cache:
             return self.lib.ct_kv8_status()
 
     def values(self, layer, seqs, s, n=None):
-        """K and V of the first n (default: all) rows of sequence s as float32 [n, kv_heads, head_dim] each."""
+        """K and V of the first n (default: all) rows of sequence s as float32 [n, kv_heads, head_dim] each;
+        rows of released pages are NaN. Without n it waits for the device, to know the length."""
         n = int(seqs.lens[s]) if n is None else n
         pages = seqs.table[s, :(n + ROWS - 1) // ROWS].long()
+        gone = (pages < 0) | (pages >= self.n_pages)
+        pages = pages.masked_fill(gone, 0)
         x = self.codes[pages, layer].view(torch.float8_e4m3fn if self.fmt == "e4m3" else torch.int8).float()
-        x = (x * self.scales[pages, layer][..., None, None]).permute(1, 0, 3, 2, 4).flatten(1, 2)[:, :n]
+        scales = self.scales[pages, layer].masked_fill(gone[:, None, None], float("nan"))
+        x = (x * scales[..., None, None]).permute(1, 0, 3, 2, 4).flatten(1, 2)[:, :n]
         return x[0], x[1]

@@ -848,6 +848,18 @@ def test_python_refuses_numbers_beyond_32_bits(kv8, torch):
     assert c.status() == 0 and torch.equal(c.refs, refs) and torch.equal(s.table, table)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_values_of_released_pages_are_nan(kv8, torch, fmt):
+    """Not those of whatever page a table entry of -1 (or one outside the pool) happens to index."""
+    c, s, rc, table = make(kv8, fmt, [70, 20], 2, 64)
+    want = c.values(1, s, 0)
+    s.table[0, 1], s.table[0, 3] = -1, c.n_pages
+    for got, w in zip(c.values(1, s, 0), want):
+        gone = torch.zeros(70, dtype=torch.bool, device="cuda")
+        gone[16:32] = gone[48:64] = True
+        assert got.shape == w.shape and bool(got[gone].isnan().all()) and torch.equal(got[~gone], w[~gone])
+
+
 def test_python_refuses_a_misaligned_pool(kv8, torch):
     arena = torch.zeros(2 * 2 * ROWS * 64 + 16, dtype=torch.uint8, device="cuda")
     scales = torch.zeros(2, 1, 2, 1, device="cuda")
