@@ -862,6 +862,7 @@ extern "C" size_t ct_kv8_pages_ws_bytes(const ct_kv8_cache *c, int n_seqs) {
 extern "C" int ct_kv8_reserve(const ct_kv8_cache *c, const ct_kv8_seqs *s, const int *add, void *ws, size_t ws_bytes,
                               void *stream) {
     if (!good_cache(c) || !c->refs || !good_seqs(s) || !add || !good_ws(ws)) return CT_EINVAL;
+    if ((long long)s->n_seqs * s->table_stride > INT_MAX) return CT_EINVAL;   // pages asked for are summed in 32 bits
     if (ws_bytes < alloc_ws(c, s->n_seqs)) return CT_ENOMEM;
     if (cudaPeekAtLastError() != cudaSuccess) return CT_EDEVICE;
     AllocArgs a = alloc_args(c, s, ws);

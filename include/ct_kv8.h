@@ -132,7 +132,7 @@ size_t ct_kv8_attn_ws_bytes(const ct_kv8_cache *c, const ct_kv8_seqs *s, int typ
 /* len[s] += add[s] (add >= 0), with pages for the new rows written into the
  * table.  When free pages run out, the sequences from the first unserved one
  * on that needs a page stay as they were (status); so does a sequence whose
- * table row is too short. */
+ * table row is too short.  n_seqs * table_stride is below 2^31. */
 int ct_kv8_reserve(const ct_kv8_cache *c, const ct_kv8_seqs *s, const int *add, void *ws, size_t ws_bytes,
                    void *stream);
 

@@ -178,6 +178,16 @@ def test_page_operators_refuse(lib, args):
     assert lib.ct_kv8_pages_ws_bytes(r, 0) == 0 and lib.ct_kv8_pages_ws_bytes(r, 65536) == 0
 
 
+def test_reserve_refuses_tables_whose_pages_do_not_count_in_32_bits(lib, args):
+    """The pages that all sequences ask for are summed in 32 bits."""
+    c, a = args.cache(), args.a
+    for n, stride in ((32, 1 << 26), (65535, 1 << 16), (65535, 1 << 26)):
+        s = args.seqs(n_seqs=n, table_stride=stride)
+        assert lib.ct_kv8_reserve(ctypes.byref(c), ctypes.byref(s), a, a, 1 << 20, None) == CT_EINVAL
+    s = args.seqs(n_seqs=31, table_stride=1 << 26)
+    assert lib.ct_kv8_reserve(ctypes.byref(c), ctypes.byref(s), a, a, 8, None) == CT_ENOMEM     # taken
+
+
 def test_ctypes_structs_match_the_header(abi, tmp_path):
     src = tmp_path / "o.c"
     fields = [("ct_kv8_cache", f) for f, _ in abi.KV8Cache._fields_] + [("ct_kv8_seqs", f) for f, _ in abi.KV8Seqs._fields_]
