@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) many_kernel(const AttnArgs a)
         const int r = TWO ? ql : i * 128 + ql, m = m0 + r;
         const float rf = sm.qf[r];
         const int t = t_first + i0 + row_of((m < M ? m : M - 1) - m0);
-        const int hi = a.causal ? min(len, t + 1) : len;   // sees j < hi and (j >= lo or j < sinks)
+        const int hi = a.causal ? max(0, min(len, t + 1)) : len;   // sees j < hi and (j >= lo or j < sinks)
         const int lo = a.window ? max(0, t - a.window + 1) : 0;
         float mref = -INFINITY, l = 0.0f, eo = E_MIN;      // O is held in units of 2^eo
         bool ok = true;
