@@ -649,7 +649,7 @@ static int pool_map(CUtensorMap *map, const Pool &p) {
 
 // ---- attention: which kernel, which tiles, which pieces
 struct AttnPlan {
-    int mt;          // few_kernel: tiles of 8 query rows per CTA; 0: many_kernel
+    int mt;          // few_kernel: MMA columns of 8 rows; 0: many_kernel
     int tile;        // query rows of a CTA
     int tiles;       // row tiles of a sequence and kv head, at most
     int chunk, max_chunks;
@@ -709,7 +709,7 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
     pl.tiles = (int)tiles;
     pl.max_chunks = (int)((list + chunk - 1) / chunk);
     if (tiles * pl.max_chunks > INT_MAX) return false;
-    // Up to 8 pieces of a tile are one cluster when all CTAs fit the SMs at once: no
+    // Up to 8 pieces of a kv head are one cluster when all CTAs fit the SMs at once: no
     // second kernel (one row over 376 keys: 1.5 us less).
     pl.cluster = pl.mt && pl.max_chunks > 1 && pl.max_chunks <= 8 && ctas * pl.max_chunks <= at_once;
     pl.ws = pl.max_chunks > 1 && !pl.cluster ? (size_t)n_rows * heads * pl.max_chunks * (c->head_dim + 2) * sizeof(float) : 0;
@@ -726,7 +726,7 @@ static int launch_few(const AttnArgs &a, const AttnPlan &pl, cudaStream_t st) {
         cudaGetLastError();
         return CT_EDEVICE;
     }
-    int rc = launch_cluster(few_kernel<T, D, FMT, MT>, dim3(pl.max_chunks * pl.tiles, a.p.heads, a.n_seqs), 128, smem, st, false,
+    int rc = launch_cluster(few_kernel<T, D, FMT, MT>, dim3(pl.max_chunks, a.p.heads, a.n_seqs), 128, smem, st, false,
                             pl.cluster ? pl.max_chunks : 1, map, a);
     if (rc == CT_OK && pl.max_chunks > 1 && !pl.cluster)
         rc = launch(join_kernel<T, D>, dim3(pl.tiles, a.p.heads, a.n_seqs), 256, 0, st, true, a, 8 * MT);

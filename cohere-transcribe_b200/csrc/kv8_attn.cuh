@@ -20,7 +20,7 @@ struct AttnArgs {
     int causal, window, sinks;
     int chunk;              // pages of a piece
     int max_chunks;
-    int cluster;            // few_kernel: the pieces of a tile are one cluster and join through its shared memory
+    int cluster;            // few_kernel: a kv head's pieces are one cluster and join through its shared memory
     float *part;            // [n_rows * heads][max_chunks][D], then [n_rows * heads][max_chunks][2]
 };
 
@@ -152,9 +152,9 @@ __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d)
 }
 
 // ---- few query rows -------------------------------------------------------------
-// One CTA per (piece of `chunk` pages, kv head and tile of 8 MT query rows,
-// sequence); the rows of a tile are (query row, head of the group) pairs, so the
-// heads that share a kv head read its codes once.  Each of the four warps takes
+// One CTA per (piece of `chunk` pages, kv head, sequence), for at most 8 MT rows: a
+// row is a (query row, head of the group) pair, so the heads that share a kv head
+// read its codes once.  Each of the four warps takes
 // every fourth page, two at a time, with an online softmax of its own; the warps
 // join through shared memory at the end.
 //
@@ -218,8 +218,7 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     extern __shared__ __align__(1024) uint8_t few_raw[];
     FewSmem<T, D, MT> &sm = *reinterpret_cast<FewSmem<T, D, MT> *>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int s = blockIdx.z, hk = blockIdx.y;
-    const int tile = a.max_chunks == 1 ? blockIdx.x : blockIdx.x / a.max_chunks, piece = blockIdx.x - tile * a.max_chunks;
+    const int s = blockIdx.z, hk = blockIdx.y, piece = blockIdx.x;
     pdl_trigger();
     if (threadIdx.x == 0) prefetch_tmap(&map);
     // Without a window the page list starts at page 0, so this lane's entry of the
@@ -233,14 +232,12 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
         if (threadIdx.x == 0 && piece == 0) set_status(CT_STATUS_BAD_ARG);
         return;
     }
-    const int G = a.group, M = sp.n * G, m0 = tile * 8 * MT;
-    if (m0 >= M) return;
-    const int i0 = m0 / G, g0 = m0 - i0 * G;   // row r of the tile: query row i0 + (g0 + r) / G, head (g0 + r) % G
+    const int G = a.group, M = sp.n * G;       // row r: query row r / G, head r % G of the group
+    if (M == 0) return;
     const float rg = __frcp_rn((float)G);
-    auto row_of = [&](int r) { return (int)((g0 + r + 0.5f) * rg); };   // exact: g0 + r < 1056
+    auto row_of = [&](int r) { return (int)((r + 0.5f) * rg); };   // exact: r < 32
     const int len = max(sp.len, 0);
-    const int t_first = len - sp.n;       // token row of query row 0 (negative: it sees nothing before row 0)
-    const int t_lo = t_first + i0, t_hi = t_first + i0 + row_of(min(8 * MT, M - m0) - 1);
+    const int t_lo = len - sp.n, t_hi = len - 1;   // token rows of the query rows (a negative one sees nothing before row 0)
     const PageList list = page_list(a, len, t_lo, t_hi);
     const int pieces = list.n <= a.chunk ? 1 : (list.n + a.chunk - 1) / a.chunk;
     if (piece >= pieces && !a.cluster) return;   // a cluster's CTAs all stay for its barriers
@@ -279,8 +276,8 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
 
     // queries -> B fragments: tile mt by warp mt
     if (warp < MT) {
-        const int mt = warp, r8 = mt * 8 + g, m = m0 + r8, qi = row_of(r8);
-        const T *qp = static_cast<const T *>(a.q) + (size_t)(sp.first + i0 + qi) * a.ldq + (size_t)(hk * G + g0 + r8 - qi * G) * D;
+        const int mt = warp, m = mt * 8 + g, qi = row_of(m);
+        const T *qp = static_cast<const T *>(a.q) + (size_t)(sp.first + qi) * a.ldq + (size_t)(hk * G + m - qi * G) * D;
         float amax = 0.0f;
         float v[KC][2][8];
 #pragma unroll
@@ -320,12 +317,12 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int m = m0 + mt * 8 + 2 * t + e;
+            const int m = mt * 8 + 2 * t + e;
             mref[mt][e] = -INFINITY;
             l[mt][e] = 0.0f;
             eo[mt][e] = E_MIN;
             qf[mt][e] = sm.qf[mt * 8 + 2 * t + e];
-            tq[mt][e] = t_first + i0 + row_of(min(m, M - 1) - m0);
+            tq[mt][e] = t_lo + row_of(min(m, M - 1));
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.0f;
@@ -576,8 +573,8 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
     __syncthreads();
     const size_t rows_all = (size_t)a.n_rows * a.heads;
     for (int i = threadIdx.x; i < 8 * MT * (D / 4); i += 128) {
-        const int row = i / (D / 4), d = (i % (D / 4)) * 4, m = m0 + row;
-        if (m >= M) continue;
+        const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (row >= M) continue;
         float mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm.m[w][row]);
@@ -598,8 +595,8 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
             if (d == 0) sm.ml[row] = make_float2(mx, lsum);
             continue;
         }
-        const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
-        const size_t r = (size_t)sp.first + i0 + qi;
+        const int qi = row_of(row), h = hk * G + row - qi * G;
+        const size_t r = (size_t)sp.first + qi;
         if (pieces == 1) {
             store4(static_cast<T *>(a.out) + r * a.ldo + (size_t)h * D + d, acc.x, acc.y, acc.z, acc.w);
         } else {
@@ -609,11 +606,11 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
         }
     }
     if (!a.cluster) return;
-    // The cluster's CTAs share out the tile's values; pieces in order.
+    // The cluster's CTAs share out the values; pieces in order.
     cluster_sync();
     for (int i = piece * 128 + threadIdx.x; i < 8 * MT * (D / 4); i += a.max_chunks * 128) {
         const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-        if (m0 + row >= M) break;
+        if (row >= M) break;
         float mc[8], lc[8], mx = -INFINITY, lsum = 0.0f;           // a cluster has 8 pieces at most
 #pragma unroll
         for (int c = 0; c < 8; ++c)
@@ -635,8 +632,8 @@ __global__ void __launch_bounds__(128, few_ctas(MT)) few_kernel(const __grid_con
                 const float4 x = dsmem_ld4(dsmem_addr(smem_u32(&sm.o[0][row][d]), c));
                 acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
             }
-        const int qi = row_of(row), h = hk * G + g0 + row - qi * G;
-        store4(static_cast<T *>(a.out) + ((size_t)sp.first + i0 + qi) * a.ldo + (size_t)h * D + d, acc.x, acc.y, acc.z, acc.w);
+        const int qi = row_of(row), h = hk * G + row - qi * G;
+        store4(static_cast<T *>(a.out) + ((size_t)sp.first + qi) * a.ldo + (size_t)h * D + d, acc.x, acc.y, acc.z, acc.w);
     }
     cluster_sync();                       // nobody leaves while its results are being read
 }
