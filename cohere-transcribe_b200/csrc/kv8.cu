@@ -874,7 +874,10 @@ extern "C" int ct_kv8_reserve(const ct_kv8_cache *c, const ct_kv8_seqs *s, const
 extern "C" int ct_kv8_fork(const ct_kv8_cache *c, const ct_kv8_seqs *src, const int *parents, const ct_kv8_seqs *dst,
                            void *ws, size_t ws_bytes, void *stream) {
     if (!good_cache(c) || !c->refs || !good_seqs(src) || !good_seqs(dst) || !parents || !good_ws(ws)) return CT_EINVAL;
-    if (src->table == dst->table || src->len == dst->len) return CT_EINVAL;
+    const auto meet = [](const int *a, size_t na, const int *b, size_t nb) { return a < b + nb && b < a + na; };
+    if (meet(src->table, (size_t)src->n_seqs * src->table_stride, dst->table, (size_t)dst->n_seqs * dst->table_stride) ||
+        meet(src->len, src->n_seqs, dst->len, dst->n_seqs))
+        return CT_EINVAL;
     if (ws_bytes < alloc_ws(c, dst->n_seqs)) return CT_ENOMEM;
     if (cudaPeekAtLastError() != cudaSuccess) return CT_EDEVICE;
     AllocArgs a = alloc_args(c, dst, ws);

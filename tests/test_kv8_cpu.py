@@ -178,6 +178,17 @@ def test_page_operators_refuse(lib, args):
     assert lib.ct_kv8_pages_ws_bytes(r, 0) == 0 and lib.ct_kv8_pages_ws_bytes(r, 65536) == 0
 
 
+@pytest.mark.parametrize("table,length", [(0, 512), (16, 512), (32, 512), (44, 512), (-44, 512), (256, 0), (256, 8), (256, -8)])
+def test_fork_refuses_sequences_that_overlap(lib, args, table, length):
+    """dst's table or lengths inside src's: three rows of four entries, three lengths."""
+    c, a = args.cache(), args.a + 1024
+    s, d = args.seqs(table=a, len=a + 2048), args.seqs(table=a + table, len=a + 2048 + length)
+    assert lib.ct_kv8_fork(ctypes.byref(c), ctypes.byref(s), args.a, ctypes.byref(d), args.a, 4096, None) == CT_EINVAL
+    for t, n in ((48, 12), (-48, -12)):                        # side by side: taken
+        d = args.seqs(table=a + t, len=a + 2048 + n)
+        assert lib.ct_kv8_fork(ctypes.byref(c), ctypes.byref(s), args.a, ctypes.byref(d), args.a, 8, None) == CT_ENOMEM
+
+
 def test_reserve_refuses_tables_whose_pages_do_not_count_in_32_bits(lib, args):
     """The pages that all sequences ask for are summed in 32 bits."""
     c, a = args.cache(), args.a
