@@ -104,8 +104,9 @@ int ct_kv8_append(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const 
  * over the rows j of r's sequence that r sees.
  * q, out: [n_rows][heads * head_dim] of `type`, row strides ldq / ldo in
  * elements; 16-byte aligned, strides a multiple of 16 bytes.  Rows belong to
- * sequences as in ct_kv8_append; row i of the n rows of sequence s is its token
- * row t = len[s] - n + i.  It sees every row j < len[s] or, with causal, those
+ * sequences as in ct_kv8_append, but with row_start NULL a sequence of length 0
+ * has its row too (which sees nothing); row i of the n rows of sequence s is its
+ * token row t = len[s] - n + i.  It sees every row j < len[s] or, with causal, those
  * with j <= t; with window > 0 (causal only) of these the ones with
  * j > t - window or j < sinks.  A row that sees nothing gets zeros.  Rows of
  * out that belong to no sequence are left as they were.
@@ -113,10 +114,16 @@ int ct_kv8_append(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const 
  * (when one is exceeded that sequence's rows of out are left as they were: status).
  * Products, sums and the softmax are fp32; K and V codes enter them exactly,
  * queries and probabilities as fp16 numbers scaled by powers of two: two each
- * (22 bits) for fp32 rows, one (11 bits, which holds a bf16 query exactly) for
- * bf16 rows.  A result depends on the sizes of the call, not on the other
- * sequences' contents, and is the same each time.  out may be q itself.
- * ws: at least ct_kv8_attn_ws_bytes of the same arguments. */
+ * (22 bits) for fp32 rows, one (11 bits) for bf16 rows.  What lies far below a
+ * row's largest keeps fewer: a query's elements are exact to 2^-25 of its largest
+ * (so bf16 ones are held exactly down to 2^-17 of it), products of probability and
+ * V scale to 2^-33 of the row's largest such product.  A query with an infinity or a
+ * NaN gives a row of NaN.  A result depends on the sizes of the call (n_seqs,
+ * max_rows, max_len, heads: they decide how the keys are cut into pieces), not on
+ * the other sequences' contents, and is the same each time.  out may be q itself.
+ * ws: at least ct_kv8_attn_ws_bytes of the same arguments.  It is n_rows * heads *
+ * (head_dim + 2) floats for each piece that the bounds max_rows and max_len allow for:
+ * a gigabyte and more for long fp32 prompts, none for most short calls. */
 int ct_kv8_attn(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const void *q, int ldq, void *out, int ldo,
                 int type, int n_rows, const int *row_start, int max_rows, int max_len, int heads, float scale,
                 int causal, int window, int sinks, void *ws, size_t ws_bytes, void *stream);
