@@ -695,9 +695,10 @@ static bool attn_plan(AttnPlan &pl, const ct_kv8_cache *c, const ct_kv8_seqs *s,
         // The tensor core truncates each of its fp32 sums, so an error grows with the
         // keys summed into one accumulator.  fp32 results take at most 1024 keys a
         // piece (1280 where that saves cutting, a sixteenth of them past 16,384) and
-        // join the pieces with rounded sums: 4 of 1842 drawn calls are further from 64
-        // bits than 1e-6 and 1.5 times torch's fp32 products, with pieces of 2048 keys
-        // 24 of 1412 (4 prompts of 1000 to 4097 rows take 2605 us instead of 2066).
+        // join the pieces with rounded sums: 14 of 12,289 fp32 calls drawn from
+        // perf/operators.py (more than 16 rows per kv head) are further from 64 bits than
+        // 1e-6 and 1.5 times their plain form, with pieces of 2048 keys 24 of 1412 were
+        // (4 prompts of 1000 to 4097 rows take 2605 us instead of 2066).
         if (type == CT_KV8_F32 && list > 80) pieces = std::max(pieces, std::min(16ll, (list + 63) / 64));
         // However long the cache, 16,384 keys a piece (bf16 results 65,536): a step loses
         // up to 2^-22 of a sum, so 2^-12 (2^-10) of it at most.

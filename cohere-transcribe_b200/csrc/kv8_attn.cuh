@@ -177,9 +177,10 @@ __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d)
 // banks.
 //
 // Bound by HBM where there is much to read (16 rows of 32 heads over 8k to 65k keys:
-// 1.19 GB in 206 us, 5.8 TB/s), otherwise by latency: a pair of pages takes a warp
-// 3 to 4 thousand cycles among 16 warps, and start and join about 6 thousand (64
-// fp32 rows over up to 1024 keys: 33 us for 62 MB; one row over 376 keys: 10.3 us).
+// 1.19 GB in 206 us, 5.8 TB/s), otherwise by instructions and latency: a pair of pages
+// takes a warp 3 to 4 thousand cycles among 16 warps, and start and join about 6
+// thousand (64 fp32 rows over up to 1024 keys: 31 us for 62 MB, 36% of the issue slots
+// at 11 warps per SM; one row over 376 keys: 10.3 us).
 // Pages in flight per warp, and CTAs per SM.  8 rows of 128 dims: 3 pages and 4
 // CTAs are 2 to 3% faster than 4 pages and 3 CTAs (attention of 16 rows over 8k to
 // 65k keys 207.5 against 213.2 us).

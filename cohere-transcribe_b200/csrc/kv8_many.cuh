@@ -28,11 +28,12 @@
 // P [128 x 128] fp16 replaces S in TMEM as the A operand: the 32 columns of 32
 // scores hold their high parts in the first 16 and their low parts in the rest.
 //
-// Measured: 4 prompts of 1000 to 4097 bf16 rows, 32 heads on 8, 679 GFLOP in 897 us
-// (757 TFLOP/s); windowed fp32 prompts, 62 GFLOP (every product as two MMAs), 276
-// us.  No unit is the bound (tensor pipe 38%, exponentials 39%, issue slots 42%): a
-// stream's chain is, about 3.1 thousand cycles of softmax and 2 thousand until its
-// next scores are there, per tile of 128 keys.  128 keys a tile keep the chain's
+// Measured: 4 prompts of 1000 to 4097 bf16 rows, 32 heads on 8, 679 GFLOP in 955 us
+// (711 TFLOP/s; 24 us of it for waiting with Q.K until P.V is finished); windowed fp32
+// prompts, 62 GFLOP (every product as two MMAs), 281 us.  No unit is the bound (tensor
+// pipe 34%, exponentials 37%, issue slots 41%): a stream's chain is, about 3.1
+// thousand cycles of softmax and over 2 thousand until its next scores are there, per
+// tile of 128 keys.  128 keys a tile keep the chain's
 // fixed part small; the straight-line softmax with all scores in registers replaced
 // loops over 32 of them (1450 us).
 #pragma once
