@@ -119,8 +119,8 @@ int ct_kv8_append(const ct_kv8_cache *c, int layer, const ct_kv8_seqs *s, const 
  * (so bf16 ones are held exactly down to 2^-17 of it), products of probability and
  * V scale to 2^-33 of the row's largest such product, and a probability below 2^-96
  * of the largest may count as 0.  A query with an infinity or a NaN gives a row of
- * NaN.  A result depends on the sizes of the call (n_seqs, max_rows, max_len,
- * heads: they decide how the keys are cut into pieces), not on
+ * NaN.  A result depends on the sizes of the call (n_seqs, table_stride, max_rows,
+ * max_len, heads, window, sinks: they decide how the keys are cut into pieces), not on
  * the other sequences' contents, and is the same each time.  out may be q itself.
  * ws: at least ct_kv8_attn_ws_bytes of the same arguments.  It is n_rows * heads *
  * (head_dim + 2) floats for each piece that the bounds max_rows and max_len allow for:
